@@ -57,8 +57,21 @@ _SIGS = {
     "dsb_pack_quant_weight": [c_p, c_i64, c_i, c_p, c_i64, c_p, c_i, c_i, c_i, c_i, c_p, c_p],
     "dsb_linear_rows": [c_p, c_i64, c_p, c_i64, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_i, c_p, c_i64, c_p, c_i64, c_p, c_p],
     "dsb_linear_static": [c_p, c_i64, c_p, c_i64, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_i, c_p, c_i64, c_p, c_p],
+    "dsb_int4_quantize": [c_p, c_i64, c_i, c_i, c_i, c_i, c_p, c_i64, c_p, c_p, c_p],
+    "dsb_int4_from_gguf": [c_i, c_p, c_i64, c_i, c_i, c_p, c_i64, c_p, c_p, c_p],
+    "dsb_int4_pack": [c_p, c_i64, c_p, c_p, c_i64, c_i, c_i, c_i, c_p, c_p, c_p, c_p],
+    "dsb_int4_dequant": [c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_i64, c_p],
+    "dsb_gemv_int4": [c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_i64, c_i, c_p, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_p],
+    "dsb_kv_append": [c_p] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_i, c_i, c_p, c_i64, c_i, c_p, c_i, c_p, c_p, c_i, c_i, c_p, c_p],
+    "dsb_kv_read": [c_p, c_p, c_i64, c_i, c_i, c_i, c_i] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_p, c_p],
+    "dsb_kv_attn_workspace_bytes": [],
+    "dsb_kv_attn": [c_p] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_i, c_i, c_i, c_p, c_i64, c_i, c_p, c_i, c_i, c_f, c_p, c_i64, c_p, c_p],
 }
 
+
+class KVCacheArgs(ctypes.Structure):
+    """``dsb_kv_cache`` of include/dsb.h."""
+    _fields_ = [("k", c_p), ("v", c_p), ("k_exp", c_p), ("v_exp", c_p), ("n_pages", c_i), ("heads", c_i), ("page_tokens", c_i)]
 
 
 class GemmArgs(ctypes.Structure):
@@ -98,7 +111,7 @@ def lib():
         for name, args in _SIGS.items():
             fn = getattr(handle, name)
             fn.argtypes = args
-            fn.restype = c_i64 if name == "dsb_flash_attn_workspace_bytes" else c_i
+            fn.restype = c_i64 if name.endswith("_workspace_bytes") else c_i
         _lib = handle
     return _lib
 

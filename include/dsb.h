@@ -396,6 +396,93 @@ int dsb_linear_static(const void* x, int64_t ld_x, const void* Wq, int64_t ld_w,
                       const float* w_scale, int w_scale_stride, const float* bias, int act, void* out,
                       int64_t ld_out, int* status, void* stream);
 
+/*
+ * Linears with 4-bit weights: code c in 0..15 of row n and column k stands for s * (c - 8), or s * c + m where the weight has
+ * minima, with one fp16 s (and m) per row and `group` consecutive columns (32, 64 or 128; the last group may be short).
+ * K is even.  codes: two per byte, the even column in the low nibble, [N, ld_codes]; scales, mins: fp16 [N, ceil(K / group)].
+ * The GGUF formats Q4_0, Q4_1 and Q4_K (utils/gguf.py:222-247,300-314) are such weights; the reference dequantises them to 16
+ * bits in every call.
+ *
+ * dsb_int4_quantize: W [N, ld_w] (fp32 or bf16) -> codes, scales (and mins, if not NULL: s = (max - min) / 15, m = min;
+ * else s = amax / 7).  dsb_int4_from_gguf: the rows of a GGUF tensor (ggml type number 2, 3 or 12; group 32) -> the same
+ * arrays; mins is NULL for Q4_0 and given for the others.
+ */
+int dsb_int4_quantize(const void* W, int64_t ld_w, int w_bf16, int N, int K, int group, uint8_t* codes, int64_t ld_codes,
+                      void* scales, void* mins, void* stream);
+int dsb_int4_from_gguf(int qtype, const uint8_t* raw, int64_t row_bytes, int N, int K, uint8_t* codes, int64_t ld_codes,
+                       void* scales, void* mins, void* stream);
+
+/*
+ * Lays such a weight out for the kernels below, once: payload of ceil(N/16) * ceil(K/64) * 512 bytes (16-byte aligned);
+ * out_scales (and out_mins) of ceil(N/16) * T * 16 * P fp16 values, with T = ceil(K/64), P = 2 for groups of 32, P = 1 for 64,
+ * and T = ceil(K/128), P = 1 for 128 (8-byte aligned).  ld_scales: of scales and mins.
+ */
+int dsb_int4_pack(const uint8_t* codes, int64_t ld_codes, const void* scales, const void* mins, int64_t ld_scales, int N, int K,
+                  int group, void* payload, void* out_scales, void* out_mins, void* stream);
+
+/* The laid-out weight as bf16 [N, ld_out]: the fp32 value s * (c - 8) or s * c + m, rounded. */
+int dsb_int4_dequant(const void* payload, const void* scales, const void* mins, int N, int K, int group, void* out, int64_t ld_out,
+                     void* stream);
+
+/*
+ * y = act_out(W . act_in(x) + bias) (+ y before, with `accumulate`) for M <= DSB_INT4_MAX_ROWS rows x[M, ld_x] (fp32 or bf16; any
+ * alignment of its type) and a laid-out 4-bit W; products and sums in fp32; y fp32 or bf16.  act_in is NONE or SILU.  y must
+ * not overlap x.
+ */
+#define DSB_INT4_MAX_ROWS 32
+int dsb_gemv_int4(const void* payload, const void* scales, const void* mins, int N, int K, int group, const void* x, int64_t ld_x,
+                  int x_bf16, const float* bias, void* y, int64_t ld_y, int y_bf16, int M, int act_in, int act_out, int accumulate,
+                  void* stream);
+
+/*
+ * Paged 8-bit cache of keys and values: k and v are e4m3 [n_pages, heads, page_tokens, 128] (contiguous, 128-byte aligned), k_exp
+ * and v_exp one int8 per page and head: the values of that block are e4m3 * 2^exp.  page_tokens is 16, 32, 64 or 128, and
+ * n_pages * heads * page_tokens is below 2^31.  `table` [B, ld_table] int32 names the `width` pages of each sequence in order.
+ *
+ * A table entry that is no page, a length or position outside the table or the rotation table: nothing is read or written
+ * there (its keys count as masked, its rows are not appended, it reads as zeros) and *status becomes DSB_ERR_ARG.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int8_t* k_exp;
+  int8_t* v_exp;
+  int n_pages, heads, page_tokens;
+} dsb_kv_cache;
+
+/*
+ * Appends rows 0..counts[b]-1 (counts NULL: all n) of k, v [B, n, heads, 128] (bf16, strides in elements, multiples of 8) to the
+ * sequences, from position start[b] (start NULL: start_all) on.  With rope (fp32 [rope_rows, 64, 2] = (cos, sin), row rope_row0
+ * + position) neighbouring columns of k are rotated on the way: (x0 c - x1 s, x0 s + x1 c), every operation rounded to fp32.
+ * Exponent of a block that receives rows: n(a) = the least e in -64..64 with a <= 448 * 2^e for the largest finite magnitude a
+ * of those rows.  Where they begin at the page's first token the block is new and takes n(a); else it takes the larger of
+ * n(a) and its own, and its earlier rows are rounded again if that grew.  Infinities become +-448 * 2^e.  What lies behind
+ * the last appended row of a page is left as it is.  A page must not be appended to twice in one call.
+ * The rotation is that of models/flux/flux_dit.py:154-159 and models/wan/wan_dit.py:54-58; the reference keeps no cache.
+ */
+int dsb_kv_append(const dsb_kv_cache* cache, const void* k, int64_t k_stride_b, int64_t k_stride_s, int64_t k_stride_h,
+                  const void* v, int64_t v_stride_b, int64_t v_stride_s, int64_t v_stride_h, int B, int n, const int32_t* table,
+                  int64_t ld_table, int width, const int32_t* start, int start_all, const int32_t* counts, const float* rope,
+                  int rope_rows, int rope_row0, int* status, void* stream);
+
+/* Tokens first .. first + n - 1 of each sequence as bf16 k, v [B, n, heads, 128] (exact). */
+int dsb_kv_read(const dsb_kv_cache* cache, const int32_t* table, int64_t ld_table, int width, int B, int first, int n, void* k,
+                int64_t k_stride_b, int64_t k_stride_s, int64_t k_stride_h, void* v, int64_t v_stride_b, int64_t v_stride_s,
+                int64_t v_stride_h, int* status, void* stream);
+
+/*
+ * o = softmax(q . k^T * sm_scale) . v of q [B, Sq, H, 128] over the first lens[b] (lens NULL: len_all) tokens of each sequence;
+ * query head h reads cache head h / (H / heads).  causal: query i sees the keys up to position lens[b] - Sq + i.  A query that
+ * sees no key gives zeros.  workspace: dsb_kv_attn_workspace_bytes() bytes, 16-byte aligned, for the partial results of sequences
+ * that are cut along their keys; calls that may run at the same time need one each.
+ * Stands beside dsb_flash_attn (models/wan/wan_dit.py:18-22,143-149), whose keys and values are bf16 rows.
+ */
+int64_t dsb_kv_attn_workspace_bytes(void);
+int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_s, int64_t q_stride_h, void* o,
+                int64_t o_stride_b, int64_t o_stride_s, int64_t o_stride_h, int B, int Sq, int H, const int32_t* table,
+                int64_t ld_table, int width, const int32_t* lens, int len_all, int causal, float sm_scale, void* workspace,
+                int64_t workspace_bytes, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -238,59 +238,459 @@ __device__ __forceinline__ float act_apply(float v, int act) {
   }
 }
 
-// One warp per row block and activation row, fp32 products.
-__global__ void __launch_bounds__(256) gemv_int4_kernel(Int4Dims d, GemvInt4 p) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Eight codes of a word as four pairs of fp16 numbers c - 8 (or c), exact: a code in the mantissa of 1024 is 1024 + c in its low four
+// bits and 1024 + 16 c in the next four, so that one shift serves four pairs.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {  // one instruction; the compiler makes two of it
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
+template <bool UNSIGNED>
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&a)[4]) {
+  constexpr uint32_t k1024 = 0x64006400u, kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+  const __half2 low = __float2half2_rn(UNSIGNED ? -1024.f : -1032.f), high = __float2half2_rn(UNSIGNED ? -64.f : -72.f), sixteenth = __float2half2_rn(0.0625f);
+  auto h2 = [](uint32_t u) { return *reinterpret_cast<const __half2*>(&u); };
+  auto u32 = [](__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); };
+  a[0] = u32(__hadd2(h2(and_or(w, kLow, k1024)), low));
+  a[1] = u32(__hfma2(h2(and_or(w, kHigh, k1024)), sixteenth, high));
+  w >>= 8;
+  a[2] = u32(__hadd2(h2(and_or(w, kLow, k1024)), low));
+  a[3] = u32(__hfma2(h2(and_or(w, kHigh, k1024)), sixteenth, high));
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// The weights stream through registers once, 512 bytes of a tile per load of a warp, and are multiplied by the tensor cores:
+// A = 16 rows x 16 columns of codes (exact in fp16), B = the activation rows as columns of fp16, fp32 sums of one group at a
+// time, which are then multiplied by the group's scale and added up in fp32.  Without minima A holds c - 8; with them it holds
+// c, and each group adds m * (sum of its activations).
+//
+// The activations keep their precision: a row is scaled by a power of two that brings its largest magnitude to [2^13, 2^14).  A
+// bf16 value is then exact in fp16 unless it is less than 2^-27 of that; an fp32 value (and a bf16 one behind an activation)
+// becomes two columns (SPLIT), high = fp16(x) and low = fp16(x - high), which leaves out 2^-23 of it at most, what one fp32
+// rounding of a product would.
+//
+// Split: a cluster of `n_share` CTAs owns a range of row blocks, each CTA a share of the columns, whose activations are all that
+// it stages; a warp takes every eighth row block of the range and streams its tiles without a pause from one to the next.
+// Shares meet in shared memory (CLUSTERED), in a fixed order.
+constexpr int kGemvSmemMax = 227 * 1024 - 1024;
+constexpr int kGemvCtas = 2;  // per SM
+constexpr int kBatch = 4;  // tiles of a warp in one of the two register buffers that the loads in flight fill
+
+__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(smem_u32(p), rank)));
+  return v;
+}
+
+template <int NT, bool SPLIT, int GROUP, bool MINS, bool CLUSTERED>
+__global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, GemvInt4 p, int n_share, int share_tiles, int round_blocks) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kRows = NT * (SPLIT ? 4 : 8);  // activation rows that the columns of B have room for
+  constexpr int kHalves = GROUP == 32 ? 2 : 1;  // groups of a tile
+  constexpr int kScaleBytes = 32 * kHalves;     // of a tile (of two tiles for groups of 128)
+  const int cols = p.M * (SPLIT ? 2 : 1);
+  // a row's pitch is 64 bytes above a multiple of 128: the 16-byte reads of two neighbouring columns share no bank
+  const int x_pitch = share_tiles * 128 + 64;
+  const int share_groups = MINS ? (share_tiles * 64 + GROUP - 1) / GROUP : 0;
+  uint8_t* xs = smem;                                               // [cols] rows of fp16
+  float* xsum = reinterpret_cast<float*>(xs + cols * x_pitch);      // [share_groups][kRows]
+  float* red = xsum + kRows * share_groups;                         // CLUSTERED: [round_blocks][M][16 rows]
+  __shared__ uint32_t amax_bits[kRows];
+  __shared__ float2 up[kRows];  // the power of two that a row's sums are multiplied by, as two factors
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = CLUSTERED ? cluster_ctarank() : 0;
+  const int n_ranges = CLUSTERED ? gridDim.x / n_share : gridDim.x, range = CLUSTERED ? blockIdx.x / n_share : blockIdx.x;
+  if (tid < kRows) amax_bits[tid] = 0;
   grid_wait();
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, m = blockIdx.y;
-  const float* xf = reinterpret_cast<const float*>(p.x) + m * p.ld_x;
-  const __nv_bfloat16* xb = reinterpret_cast<const __nv_bfloat16*>(p.x) + m * p.ld_x;
-  for (int rb = blockIdx.x * 8 + (threadIdx.x >> 5); rb < d.row_blocks; rb += gridDim.x * 8) {
-    float acc[2] = {0.f, 0.f};
-    for (int kt = 0; kt < d.k_tiles; ++kt) {
-      const uint4 q = p.payload[(static_cast<int64_t>(rb) * d.k_tiles + kt) * 32 + lane];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const int tile0 = rank * share_tiles;
+  const int n_tiles = max(0, min(share_tiles, d.k_tiles - tile0));   // of this share in every row block
+  const int block0 = static_cast<int>(static_cast<int64_t>(d.row_blocks) * range / n_ranges);
+  const int block1 = static_cast<int>(static_cast<int64_t>(d.row_blocks) * (range + 1) / n_ranges);
+
+  uint4 w[2][kBatch];
+  uint2 sc[2][kBatch], mn[2][kBatch];
+  // the next tile that this warp requests: its payload, its scales, its number in the share
+  const uint4* pw;
+  const uint8_t* ps;
+  int ahead, left;   // ... and how many tiles of the round are not requested yet
+  const int64_t min_off = MINS ? reinterpret_cast<const uint8_t*>(p.mins) - reinterpret_cast<const uint8_t*>(p.scales) : 0;
+  const int64_t w_jump = (static_cast<int64_t>(d.k_tiles) * 8 - n_tiles) * 32;
+  const int64_t s_jump = static_cast<int64_t>(d.scale_tiles) * 8 * kScaleBytes;
+  auto load_one = [&](int buf, int u, const uint4* from, int kt) {
+    w[buf][u] = load_stream(from);
+    const uint8_t* at = ps + (GROUP == 128 ? kt >> 1 : kt) * kScaleBytes;
+    if constexpr (GROUP == 32) {
+      sc[buf][u] = __ldg(reinterpret_cast<const uint2*>(at));
+      if constexpr (MINS) mn[buf][u] = __ldg(reinterpret_cast<const uint2*>(at + min_off));
+    } else {
+      sc[buf][u].x = __ldg(reinterpret_cast<const uint32_t*>(at));
+      if constexpr (MINS) mn[buf][u].x = __ldg(reinterpret_cast<const uint32_t*>(at + min_off));
+    }
+  };
+  auto load = [&](int buf) {
+    if (left >= kBatch && ahead + kBatch <= n_tiles) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = kt * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1);
-        float x[4];
+      for (int u = 0; u < kBatch; ++u) load_one(buf, u, pw + u * 32, ahead + u);
+      pw += kBatch * 32;
+      ahead += kBatch;
+      if (ahead == n_tiles) ahead = 0, pw += w_jump, ps += s_jump;
+    } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          x[c] = 0.f;
-          if (k + c < d.K) x[c] = p.x_bf16 ? __bfloat162float(xb[k + c]) : xf[k + c];
-          if (p.act_in == DSB_ACT_SILU) x[c] = silu(x[c]);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int64_t si = scale_index(d, rb, g + 8 * r, k);
-          const float s = __half2float(p.scales[si]);
-          float a = 0.f, sum = 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            a += (static_cast<float>((w[j] >> (4 * (r + 2 * (c >> 1) + 4 * (c & 1)))) & 15u) - 8.f) * x[c];
-            sum += x[c];
-          }
-          acc[r] += s * a;
-          if (p.mins) acc[r] += (__half2float(p.mins[si]) + 8.f * s) * sum;
+      for (int u = 0; u < kBatch; ++u) {
+        if (u < left) {
+          load_one(buf, u, pw, ahead);
+          pw += 32;
+          if (++ahead == n_tiles) ahead = 0, pw += w_jump, ps += s_jump;
         }
       }
     }
+    left -= kBatch;
+  };
+  auto begin = [&](int first_block, int blocks) {
+    const int mine = blocks > warp ? (blocks - warp - 1) / 8 + 1 : 0;
+    const int64_t rb = first_block + warp;
+    left = mine * n_tiles;
+    ahead = 0;
+    pw = p.payload + (rb * d.k_tiles + tile0) * 32 + lane;
+    ps = reinterpret_cast<const uint8_t*>(p.scales) + (rb * d.scale_tiles + (GROUP == 128 ? tile0 >> 1 : tile0)) * kScaleBytes +
+         g * (kScaleBytes / 8);
+    load(0);
+    load(1);
+  };
+  int round0 = block0, in_round = min(round_blocks, block1 - block0);
+  begin(round0, in_round);
+
+  // ---- the activations of this share
+  auto eight = [&](int m, int e8, float (&v)[8]) {  // eight neighbouring columns of a row; columns past the last are zero
+    const int k = tile0 * 64 + e8 * 8;
+    const int64_t off = m * p.ld_x + k;
+    const uint8_t* at = reinterpret_cast<const uint8_t*>(p.x) + off * (p.x_bf16 ? 2 : 4);
+    if (k + 8 <= d.K && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at);
+      if (!p.x_bf16) {
+        const uint4 b = *reinterpret_cast<const uint4*>(at + 16);
+        v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+      } else {
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 1);
-      acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 2);
-      const int n = rb * 16 + g + 8 * r;
-      if (t == 0 && n < d.N) {
-        float v = act_apply(acc[r] + (p.bias ? p.bias[n] : 0.f), p.act_out);
-        if (p.y_bf16) {
-          __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + m * p.ld_y + n;
-          *y = __float2bfloat16_rn(p.accumulate ? v + __bfloat162float(*y) : v);
-        } else {
-          float* y = reinterpret_cast<float*>(p.y) + m * p.ld_y + n;
-          *y = p.accumulate ? v + *y : v;
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack_bf16x2(u[j]);
+          v[2 * j] = f.x, v[2 * j + 1] = f.y;
         }
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = 0.f;
+        if (k + j < d.K)
+          v[j] = p.x_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.x)[off + j]) : reinterpret_cast<const float*>(p.x)[off + j];
+      }
+    }
+    if (SPLIT && p.act_in == DSB_ACT_SILU) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = silu(v[j]);
+    }
+  };
+  auto largest = [&](int m, const float (&v)[8]) {  // of a warp's finite magnitudes, into the row's
+    float a = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (fabsf(v[j]) < INFINITY) a = fmaxf(a, fabsf(v[j]));
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
+    if (lane == 0) atomicMax(&amax_bits[m], bits);
+  };
+  auto convert = [&](int m, int e8, bool in, const float (&v)[8]) {
+    // the power of two, as two factors: its exponent may pass 127
+    const uint32_t top = amax_bits[m];
+    const int e = top ? ilogbf(__uint_as_float(top)) - 13 : 0, half = e / 2;
+    const float f0 = pow2f(-half), f1 = pow2f(half - e);
+    uint32_t hi[4], lo[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = v[2 * j] * f0 * f1, b = v[2 * j + 1] * f0 * f1;
+      const __half2 h = __floats2half2_rn(a, b);
+      hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+      sum += a + b;
+      if constexpr (SPLIT) {
+        // (an infinity is its high part alone)
+        const float ra = fabsf(a) < INFINITY ? a - __low2float(h) : 0.f, rb = fabsf(b) < INFINITY ? b - __high2float(h) : 0.f;
+        const __half2 l = __floats2half2_rn(ra, rb);
+        lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+      }
+    }
+    uint8_t* at = xs + (SPLIT ? 2 * m : m) * x_pitch + e8 * 16;
+    if (in) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (SPLIT) *reinterpret_cast<uint4*>(at + x_pitch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    if constexpr (MINS) {
+#pragma unroll
+      for (int o = 1; o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (in && (lane & (GROUP / 8 - 1)) == 0) xsum[e8 / (GROUP / 8) * kRows + m] = sum;
+    }
+  };
+  {
+    const int eights = n_tiles * 8, spans = (eights + 31) / 32, units = p.M * spans;  // a unit: 32 x 8 columns of one row
+    __syncthreads();
+#pragma unroll 1
+    for (int u = warp; u < units; u += 8) {
+      const int m = u / spans, e8 = (u - m * spans) * 32 + lane;
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (e8 < eights) eight(m, e8, x);
+      largest(m, x);
+    }
+    __syncthreads();
+    if (tid < p.M) {
+      const int e = amax_bits[tid] ? ilogbf(__uint_as_float(amax_bits[tid])) - 13 : 0, half = e / 2;
+      up[tid] = make_float2(pow2f(half), pow2f(e - half));
+    }
+#pragma unroll 1
+    for (int u = warp; u < units; u += 8) {
+      const int m = u / spans, e8 = (u - m * spans) * 32 + lane;
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (e8 < eights) eight(m, e8, x);
+      convert(m, e8, e8 < eights, x);
+    }
+    __syncthreads();
+  }
+
+  // ---- products
+  // Lanes whose column of B is not there read the last one's: what it gives is never looked at.
+  const uint8_t* xb[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) xb[n] = xs + min(n * 8 + g, cols - 1) * x_pitch + t * 16;
+  float acc[NT][4];
+  auto tile = [&](const uint4& q, const uint2& s2, const uint2& m2, int kt) {
+    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+    float c[NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 b[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) b[n] = *reinterpret_cast<const uint4*>(xb[n] + kt * 128 + h * 64);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t a[4];
+        codes_to_f16<MINS>(words[2 * h + j], a);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (j == 0 && (h == 0 || GROUP == 32))
+            mma_f16_first(c[n], a, b[n].x, b[n].y);
+          else
+            mma_f16(c[n], a, j ? b[n].z : b[n].x, j ? b[n].w : b[n].y);
+        }
+      }
+      if (h == 1 || GROUP == 32) {
+        const uint32_t sw = GROUP == 32 && h == 1 ? s2.y : s2.x;
+        const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sw));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = fmaf(s.x, c[n][0], acc[n][0]);
+          acc[n][1] = fmaf(s.x, c[n][1], acc[n][1]);
+          acc[n][2] = fmaf(s.y, c[n][2], acc[n][2]);
+          acc[n][3] = fmaf(s.y, c[n][3], acc[n][3]);
+        }
+        if (MINS && (GROUP != 128 || (kt & 1) == 0)) {  // a group that spans two tiles adds its minimum's term with the first
+          const int grp = GROUP == 32 ? kt * 2 + h : GROUP == 64 ? kt : kt >> 1;
+          const uint32_t mw = GROUP == 32 && h == 1 ? m2.y : m2.x;
+          const float2 mv = __half22float2(*reinterpret_cast<const __half2*>(&mw));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (SPLIT) {
+              const float x0 = xsum[grp * kRows + n * 4 + t];
+              acc[n][0] = fmaf(mv.x, x0, acc[n][0]);
+              acc[n][2] = fmaf(mv.y, x0, acc[n][2]);
+            } else {
+              const float2 x2 = *reinterpret_cast<const float2*>(xsum + grp * kRows + n * 8 + 2 * t);
+              acc[n][0] = fmaf(mv.x, x2.x, acc[n][0]);
+              acc[n][1] = fmaf(mv.x, x2.y, acc[n][1]);
+              acc[n][2] = fmaf(mv.y, x2.x, acc[n][2]);
+              acc[n][3] = fmaf(mv.y, x2.y, acc[n][3]);
+            }
+          }
+        }
+      }
+    }
+  };
+  auto emit = [&](int m, int n, float v) {
+    v = act_apply(v + (p.bias ? p.bias[n] : 0.f), p.act_out);
+    if (p.y_bf16) {
+      __nv_bfloat16* y = reinterpret_cast<__nv_bfloat16*>(p.y) + m * p.ld_y + n;
+      *y = __float2bfloat16_rn(p.accumulate ? v + __bfloat162float(*y) : v);
+    } else {
+      float* y = reinterpret_cast<float*>(p.y) + m * p.ld_y + n;
+      *y = p.accumulate ? v + *y : v;
+    }
+  };
+  // the sums of a finished row block (its number in the round)
+  auto finish = [&](int block) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < (SPLIT ? 1 : 2); ++c) {
+          const int m = SPLIT ? n * 4 + t : n * 8 + 2 * t + c, row = g + 8 * r;
+          if (m < p.M) {
+            const float v = (SPLIT ? acc[n][2 * r] + acc[n][2 * r + 1] : acc[n][2 * r + c]) * up[m].x * up[m].y;
+            if constexpr (CLUSTERED)
+              red[(block * p.M + m) * 16 + row] = v;
+            else if ((round0 + block) * 16 + row < d.N)
+              emit(m, (round0 + block) * 16 + row, v);
+          }
+        }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  };
+
+  for (;;) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    int kt = 0, block = warp;
+    // (a share without tiles: its sums are zero)
+    if (n_tiles == 0)
+      for (; block < in_round; block += 8) finish(block);
+    int todo = block < in_round ? ((in_round - block - 1) / 8 + 1) * n_tiles : 0;
+    auto multiply = [&](int buf) {
+      if (todo >= kBatch && kt + kBatch <= n_tiles) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) tile(w[buf][u], sc[buf][u], mn[buf][u], kt + u);
+        kt += kBatch;
+        if (kt == n_tiles) finish(block), kt = 0, block += 8;
+      } else {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (u < todo) {
+            tile(w[buf][u], sc[buf][u], mn[buf][u], kt);
+            if (++kt == n_tiles) finish(block), kt = 0, block += 8;
+          }
+        }
+      }
+      todo -= kBatch;
+    };
+    while (todo > 0) {
+      multiply(0);
+      load(0);
+      multiply(1);
+      load(1);
+    }
+    const int next = round0 + in_round, next_in = min(round_blocks, block1 - next);
+    if constexpr (CLUSTERED) {
+      cluster_sync_all();
+      if (next_in > 0) {
+        begin(next, next_in);
+      }
+      const int total = in_round * p.M * 16;
+      for (int i = rank * 256 + tid; i < total; i += n_share * 256) {
+        const int row = i & 15, bm = i >> 4, m = bm % p.M, n = (round0 + bm / p.M) * 16 + row;
+        if (n < d.N) {
+          float v = 0.f;
+          for (int r = 0; r < n_share; ++r) v += ld_cluster(red + i, r);
+          emit(m, n, v);
+        }
+      }
+      cluster_sync_all();   // nobody reads this CTA's sums any more
+    }
+    if (next_in <= 0) break;
+    if constexpr (!CLUSTERED) {
+      begin(next, next_in);
+    }
+    round0 = next;
+    in_round = next_in;
+  }
+}
+
+template <int NT, bool SPLIT, int GROUP, bool MINS, bool CLUSTERED>
+static int run_gemv_int4(const Int4Dims& d, const GemvInt4& p, int n_share, cudaStream_t st) {
+  auto kern = gemv_int4_kernel<NT, SPLIT, GROUP, MINS, CLUSTERED>;
+  DSB_ENSURE_SMEM(kern, kGemvSmemMax);
+  int share = (d.k_tiles - 1) / n_share + 1;
+  if (GROUP == 128) share = (share + 1) & ~1;   // shares end where groups do
+  const int cols = p.M * (SPLIT ? 2 : 1), groups = MINS ? (share * 64 + GROUP - 1) / GROUP : 0;
+  const int64_t fixed = static_cast<int64_t>(cols) * (share * 128 + 64) + static_cast<int64_t>(groups) * NT * (SPLIT ? 4 : 8) * 4;
+  const int block_bytes = CLUSTERED ? p.M * 64 : 0;
+  if (fixed + 8 * block_bytes > kGemvSmemMax) return DSB_ERR_UNSUPPORTED;
+  // CTAs that run at once, and the row ranges (a CTA's, or a cluster's) that they make
+  const int fit = static_cast<int>((227 << 10) / (fixed + 8 * block_bytes + 2048));
+  const int occ = fit > kGemvCtas ? kGemvCtas : fit < 1 ? 1 : fit;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = n_share;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTERED ? 2 : 1;
+  int ranges = sm_count() * occ;
+  if (CLUSTERED) {
+    // clusters that run at once: a GPC holds whole ones, so fewer than the SMs would.  Asked once per device, occupancy and size.
+    static std::atomic<int> cached[64][kGemvCtas][4];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return DSB_ERR_CUDA;
+    std::atomic<int>& c = cached[dev][occ - 1][n_share == 8 ? 3 : n_share >> 1];
+    ranges = c.load();
+    if (ranges == 0) {
+      cfg.gridDim = dim3(sm_count() / n_share * n_share, 1, 1);
+      cfg.dynamicSmemBytes = (227 << 10) / occ - 2048;
+      if (cudaOccupancyMaxActiveClusters(&ranges, kern, &cfg) != cudaSuccess || ranges <= 0) ranges = sm_count() * occ / n_share;
+      c.store(ranges);
     }
   }
+  const int most = (d.row_blocks - 1) / 8 + 1;
+  if (ranges > most) ranges = most;
+  const int per_range = (d.row_blocks - 1) / ranges + 1;
+  int round = per_range;
+  int64_t bytes = fixed + static_cast<int64_t>(round) * block_bytes;
+  if (CLUSTERED) {
+    const int64_t room = (227 << 10) / occ - 2048;
+    if (bytes > room) {
+      round = static_cast<int>((room - fixed) / block_bytes) & ~7;
+      if (round < 8) round = 8;
+      bytes = fixed + static_cast<int64_t>(round) * block_bytes;
+    }
+  }
+  cfg.gridDim = dim3(ranges * n_share, 1, 1);
+  cfg.dynamicSmemBytes = bytes;
+  return cudaLaunchKernelEx(&cfg, kern, d, p, n_share, share, round) == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
+}
+
+template <int NT, bool SPLIT, int GROUP, bool MINS>
+static int launch_gemv_int4(const Int4Dims& d, const GemvInt4& p, cudaStream_t st) {
+  // Shares of the columns, of four tiles at least.  Each costs a CTA less staging and evens out the work, and a pass over the
+  // sums through distributed shared memory.  Measured (us; 1, 2, 4, 8 shares): 5120 x 5120 20.2 13.4 10.8 10.9, 13827 x 5104 with
+  // five rows 25.7 20.6 17.7 17.9, with 16 rows 52 35 26 25, 30720 x 5120 25.4 23.9 23.5 25.5, 491520 x 5120 261 253 269 316 and
+  // with minima 269 279 301 342.  Weights with fewer row blocks than four shares need to reach every SM take eight.
+  int n_share = d.row_blocks * 4 < 8 * sm_count() ? 8 : 4;
+  while (n_share > 1 && d.k_tiles < 4 * n_share) n_share /= 2;
+  if (d.row_blocks >= 16 * 8 * sm_count()) n_share = 1;
+  if (n_share == 1) {
+    const int rc = run_gemv_int4<NT, SPLIT, GROUP, MINS, false>(d, p, 1, st);
+    if (rc != DSB_ERR_UNSUPPORTED) return rc;
+    n_share = 8;
+  }
+  return run_gemv_int4<NT, SPLIT, GROUP, MINS, true>(d, p, n_share, st);
 }
 
 }  // namespace dsb
@@ -394,7 +794,31 @@ extern "C" int dsb_gemv_int4(const void* payload, const void* scales, const void
   p.act_in = act_in;
   p.act_out = act_out;
   p.accumulate = accumulate ? 1 : 0;
-  const cudaError_t err = launch_kernel(gemv_int4_kernel, dim3(stride_grid((d.row_blocks + 7) / 8), M), 256, 0,
-                                        reinterpret_cast<cudaStream_t>(stream), d, p);
-  return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // up to 16 columns of B at a time: 16 rows, or 8 of two columns each
+  const bool split = !x_bf16 || act_in != DSB_ACT_NONE;
+  const int most = split ? 8 : 16;
+  for (int m0 = 0; m0 < M; m0 += most) {
+    GemvInt4 q = p;
+    q.M = M - m0 < most ? M - m0 : most;
+    q.x = reinterpret_cast<const uint8_t*>(x) + m0 * ld_x * (x_bf16 ? 2 : 4);
+    q.y = reinterpret_cast<uint8_t*>(y) + m0 * ld_y * (y_bf16 ? 2 : 4);
+    const bool two = q.M * (split ? 2 : 1) > 8;
+    int rc;
+#define DSB_G4(NT, SPLIT, GROUP) \
+  rc = mins ? launch_gemv_int4<NT, SPLIT, GROUP, true>(d, q, st) : launch_gemv_int4<NT, SPLIT, GROUP, false>(d, q, st)
+#define DSB_G4_GROUP(NT, SPLIT) \
+  if (group == 32) DSB_G4(NT, SPLIT, 32); \
+  else if (group == 64) DSB_G4(NT, SPLIT, 64); \
+  else DSB_G4(NT, SPLIT, 128);
+    if (!split) {
+      if (two) { DSB_G4_GROUP(2, false) } else { DSB_G4_GROUP(1, false) }
+    } else {
+      if (two) { DSB_G4_GROUP(2, true) } else { DSB_G4_GROUP(1, true) }
+    }
+#undef DSB_G4_GROUP
+#undef DSB_G4
+    if (rc != DSB_OK) return rc;
+  }
+  return DSB_OK;
 }

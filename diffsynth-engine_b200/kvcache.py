@@ -121,6 +121,21 @@ def read(cache: PagedKVCache, table, n: int, first: int = 0):
     return k, v
 
 
+_workspace = {}
+
+
+def workspace_bytes(device) -> int:
+    """Bytes of scratch that a call of :func:`attend` on ``device`` takes (``dsb_kv_attn_workspace_bytes``)."""
+    n = _workspace.get(device.index)
+    if n is None:
+        with torch.cuda.device(device):
+            n = _workspace[device.index] = int(_lib.lib().dsb_kv_attn_workspace_bytes())
+        if n <= 0:
+            _workspace.pop(device.index)
+            raise _lib.DsbError("dsb_kv_attn_workspace_bytes failed")
+    return n
+
+
 def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=None, out=None):
     """Attention of ``q`` (bf16 ``[B, Sq, H, 128]``) over the first ``lens`` tokens (int, or int32 ``[B]``) of each sequence; H is a
     multiple of the cache's heads, query head h reads cache head ``h // (H // heads)``.  ``causal``: query i sees the keys up to
@@ -145,9 +160,10 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
             raise _lib.DsbError("out has the shape of q and a place for each of its values")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(HEAD_DIM)
+    ws = torch.empty(workspace_bytes(q.device), dtype=torch.uint8, device=q.device)
     rc = _lib.lib().dsb_kv_attn(
         cache._ref, _ptr(q), q.stride(0), q.stride(1), q.stride(2), _ptr(out), out.stride(0), out.stride(1), out.stride(2), B, Sq, H,
-        _ptr(table), ld, width, _ptr(dev_lens), 0 if dev_lens is not None else lens, 1 if causal else 0, float(sm_scale), None, 0,
-        _ptr(status_word(q.device)), _stream())
+        _ptr(table), ld, width, _ptr(dev_lens), 0 if dev_lens is not None else lens, 1 if causal else 0, float(sm_scale),
+        _ptr(ws), ws.numel(), _ptr(status_word(q.device)), _stream())
     check(rc, "dsb_kv_attn")
     return out

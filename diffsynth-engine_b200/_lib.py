@@ -60,13 +60,18 @@ _SIGS = {
     "dsb_int4_quantize": [c_p, c_i64, c_i, c_i, c_i, c_i, c_p, c_i64, c_p, c_p, c_p],
     "dsb_int4_from_gguf": [c_i, c_p, c_i64, c_i, c_i, c_p, c_i64, c_p, c_p, c_p],
     "dsb_int4_pack": [c_p, c_i64, c_p, c_p, c_i64, c_i, c_i, c_i, c_p, c_p, c_p, c_p],
-    "dsb_int4_dequant": [c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_i64, c_p],
-    "dsb_gemv_int4": [c_p, c_p, c_p, c_i, c_i, c_i, c_p, c_i64, c_i, c_p, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_p],
+    "dsb_int4_dequant": [c_p, c_p, c_i64, c_p],
+    "dsb_gemv_int4": [c_p, c_p, c_i64, c_i, c_p, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_p],
     "dsb_kv_append": [c_p] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_i, c_i, c_p, c_i64, c_i, c_p, c_i, c_p, c_p, c_i, c_i, c_p, c_p],
     "dsb_kv_read": [c_p, c_p, c_i64, c_i, c_i, c_i, c_i] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_p, c_p],
     "dsb_kv_attn_workspace_bytes": [],
     "dsb_kv_attn": [c_p] + [c_p, c_i64, c_i64, c_i64] * 2 + [c_i, c_i, c_i, c_p, c_i64, c_i, c_p, c_i, c_i, c_f, c_p, c_i64, c_p, c_p],
 }
+
+
+class Int4Args(ctypes.Structure):
+    """``dsb_int4_weight`` of include/dsb.h."""
+    _fields_ = [("payload", c_p), ("scales", c_p), ("mins", c_p), ("N", c_i), ("K", c_i), ("group", c_i)]
 
 
 class KVCacheArgs(ctypes.Structure):

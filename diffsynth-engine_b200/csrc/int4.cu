@@ -754,10 +754,11 @@ extern "C" int dsb_int4_pack(const uint8_t* codes, int64_t ld_codes, const void*
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }
 
-extern "C" int dsb_int4_dequant(const void* payload, const void* scales, const void* mins, int N, int K, int group, void* out,
-                                int64_t ld_out, void* stream) {
+extern "C" int dsb_int4_dequant(const dsb_int4_weight* w, void* out, int64_t ld_out, void* stream) {
+  if (!w) return DSB_ERR_ARG;
+  const void *payload = w->payload, *scales = w->scales, *mins = w->mins;
   Int4Dims d;
-  if (!payload || !scales || !out || !int4_dims(&d, N, K, group) || ld_out < K || !al(payload, 16) || !al(scales, 8) ||
+  if (!payload || !scales || !out || !int4_dims(&d, w->N, w->K, w->group) || ld_out < w->K || !al(payload, 16) || !al(scales, 8) ||
       !al(mins, 8) || !al(out, 2))
     return DSB_ERR_ARG;
   const int64_t words = static_cast<int64_t>(d.row_blocks) * d.k_tiles * 128;
@@ -768,9 +769,11 @@ extern "C" int dsb_int4_dequant(const void* payload, const void* scales, const v
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }
 
-extern "C" int dsb_gemv_int4(const void* payload, const void* scales, const void* mins, int N, int K, int group, const void* x,
-                             int64_t ld_x, int x_bf16, const float* bias, void* y, int64_t ld_y, int y_bf16, int M, int act_in,
-                             int act_out, int accumulate, void* stream) {
+extern "C" int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld_x, int x_bf16, const float* bias, void* y, int64_t ld_y,
+                             int y_bf16, int M, int act_in, int act_out, int accumulate, void* stream) {
+  if (!w) return DSB_ERR_ARG;
+  const void *payload = w->payload, *scales = w->scales, *mins = w->mins;
+  const int N = w->N, K = w->K, group = w->group;
   Int4Dims d;
   if (M < 0 || M > DSB_INT4_MAX_ROWS || !int4_dims(&d, N, K, group)) return DSB_ERR_ARG;
   if (act_in != DSB_ACT_NONE && act_in != DSB_ACT_SILU) return DSB_ERR_ARG;

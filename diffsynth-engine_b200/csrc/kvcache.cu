@@ -31,8 +31,10 @@ __device__ __forceinline__ float e4m3_to_float(uint32_t byte) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
   return __half2float(*reinterpret_cast<const __half*>(&h));
 }
-__device__ __forceinline__ uint32_t float_to_e4m3(float x) {
-  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 // 2^e for e in [-128, 127)
 __device__ __forceinline__ float pow2i(int e) { return e < -126 ? ldexpf(1.f, e) : __int_as_float((e + 127) << 23); }
@@ -52,11 +54,13 @@ struct KvAppend {
   int* status;
 };
 
-// One CTA per page that the rows of a sequence touch, head, and pool (k or v).
-__global__ void __launch_bounds__(128) kv_append_kernel(KvAppend p) {
+// One CTA per page that the rows of a sequence touch, head, and pool (k or v): its rows are read once, eight columns a load, kept
+// (rotated) in registers while the block's exponent is found, and written as e4m3.  CHUNKS: loads of a thread for a whole page.
+template <int THREADS, int CHUNKS>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(KvAppend p) {
   grid_wait();
-  __shared__ float red[4];
-  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, h = blockIdx.y, T = p.pool.T;
+  __shared__ uint32_t red[THREADS / 32];
+  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, h = blockIdx.y, T = p.pool.T, tid = threadIdx.x;
   const int start = p.start ? p.start[b] : p.start_all, count = p.counts ? p.counts[b] : p.n;
   const bool rotate = which == 0 && p.rope != nullptr;
   if (!kv_append_ok(start, count, p.n, p.tab.capacity(T)) ||
@@ -68,6 +72,53 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvAppend p) {
   const KvSpan s = kv_span(start, count, T, blockIdx.x);
   if (s.rows == 0) return;
   const int page = kv_page(p.tab.row(b), p.tab.width, p.pool.n_pages, s.index);
+  // (the rows are on their way while the page is looked up)
+  const __nv_bfloat16* src = p.src[which] + b * p.sb[which] + h * p.sh[which];
+  float x[CHUNKS][8];
+  uint32_t top = 0;   // largest finite magnitude, as bits
+  {
+    uint4 raw[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = tid + c * THREADS;
+      raw[c] = make_uint4(0, 0, 0, 0);
+      if (i < s.rows * 16) {
+        const __nv_bfloat16* at = src + static_cast<int64_t>(s.row + (i >> 4)) * p.sn[which] + (i & 15) * 8;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w)
+                     : "l"(at));
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = tid + c * THREADS;
+      const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = unpack_bf16x2(u[e]);
+        x[c][2 * e] = v.x, x[c][2 * e + 1] = v.y;
+      }
+      if (rotate && i < s.rows * 16) {
+        const float4* cs = reinterpret_cast<const float4*>(p.rope) +
+                           (static_cast<int64_t>(p.rope_row0) + start + s.row + (i >> 4)) * 32 + (i & 15) * 2;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 r = __ldg(cs + e);   // two pairs' (cos, sin)
+          float* v = x[c] + 4 * e;
+          const float a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
+          v[0] = __fsub_rn(__fmul_rn(a0, r.x), __fmul_rn(a1, r.y));
+          v[1] = __fadd_rn(__fmul_rn(a0, r.y), __fmul_rn(a1, r.x));
+          v[2] = __fsub_rn(__fmul_rn(a2, r.z), __fmul_rn(a3, r.w));
+          v[3] = __fadd_rn(__fmul_rn(a2, r.w), __fmul_rn(a3, r.z));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = __float_as_uint(x[c][e]) & 0x7fffffffu;
+        if (bits < 0x7f800000u) top = max(top, bits);
+      }
+    }
+  }
   if (page < 0) {
     if (p.status) *p.status = DSB_ERR_ARG;
     return;
@@ -75,44 +126,35 @@ __global__ void __launch_bounds__(128) kv_append_kernel(KvAppend p) {
   const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
   uint8_t* dst = (which ? p.pool.v : p.pool.k) + block * T * kD;
   int8_t* exps = (which ? p.pool.v_exp : p.pool.k_exp) + block;
-  const __nv_bfloat16* src = p.src[which] + b * p.sb[which] + h * p.sh[which];
-  auto pair = [&](int i) {  // the i-th pair of neighbouring columns of the rows that go to this page
-    const int r = i >> 6, c = (i & 63) * 2;
-    const __nv_bfloat16* x = src + static_cast<int64_t>(s.row + r) * p.sn[which] + c;
-    float2 v = make_float2(__bfloat162float(x[0]), __bfloat162float(x[1]));
-    if (rotate) {
-      const float2 cs =
-          reinterpret_cast<const float2*>(p.rope)[static_cast<int64_t>(p.rope_row0 + start + s.row + r) * 64 + (c >> 1)];
-      v = make_float2(__fsub_rn(__fmul_rn(v.x, cs.x), __fmul_rn(v.y, cs.y)), __fadd_rn(__fmul_rn(v.x, cs.y), __fmul_rn(v.y, cs.x)));
-    }
-    return v;
-  };
-  float amax = 0.f;
-  for (int i = threadIdx.x; i < s.rows * 64; i += 128) {
-    const float2 v = pair(i);
-    if (fabsf(v.x) < INFINITY) amax = fmaxf(amax, fabsf(v.x));
-    if (fabsf(v.y) < INFINITY) amax = fmaxf(amax, fabsf(v.y));
-  }
-  amax = warp_max(amax);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
   const int was = *exps;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) red[tid >> 5] = top;
   __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  int e = kv_exponent(__float_as_uint(amax));
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) top = max(top, red[i]);
+  int e = kv_exponent(top);
   if (s.slot > 0) {
     e = max(e, was);
     if (e > was) {
       const float fall = pow2i(was - e);
-      for (int i = threadIdx.x; i < s.slot * kD; i += 128) dst[i] = static_cast<uint8_t>(float_to_e4m3(e4m3_to_float(dst[i]) * fall));
+      for (int i = tid; i < s.slot * (kD / 4); i += THREADS) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(dst) + i;
+        const uint32_t q = *at;
+        *at = e4m3x4(e4m3_to_float(q & 255u) * fall, e4m3_to_float((q >> 8) & 255u) * fall, e4m3_to_float((q >> 16) & 255u) * fall,
+                     e4m3_to_float(q >> 24) * fall);
+      }
     }
   }
-  if (threadIdx.x == 0) *exps = static_cast<int8_t>(e);
+  if (tid == 0) *exps = static_cast<int8_t>(e);
   const float inv = pow2i(-e);
-  for (int i = threadIdx.x; i < s.rows * 64; i += 128) {
-    const float2 v = pair(i);
-    uint8_t* d = dst + s.slot * kD + 2 * i;
-    d[0] = static_cast<uint8_t>(float_to_e4m3(v.x * inv));
-    d[1] = static_cast<uint8_t>(float_to_e4m3(v.y * inv));
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = tid + c * THREADS;
+    if (i < s.rows * 16) {
+      const float* v = x[c];
+      reinterpret_cast<uint2*>(dst + s.slot * kD)[i] =
+          make_uint2(e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+    }
   }
 }
 
@@ -126,27 +168,34 @@ struct KvRead {
   int* status;
 };
 
-// One warp per (token, head) and pool; 4 columns a lane.  e4m3 * 2^e is exact in bf16.
+// Eight lanes per (token, head) and pool, 16 columns each.  e4m3 * 2^e is exact in bf16 (but below 2^-126, where it is rounded).
 __global__ void __launch_bounds__(256) kv_read_kernel(KvRead p) {
   grid_wait();
-  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, h = blockIdx.y, T = p.pool.T, lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, T = p.pool.T, c = threadIdx.x & 7;
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x >> 3);
+  const int i = static_cast<int>(x / p.pool.heads), h = static_cast<int>(x - static_cast<int64_t>(i) * p.pool.heads);
   if (i >= p.n) return;
   const int tok = p.first + i;
   const int page = kv_page(p.tab.row(b), p.tab.width, p.pool.n_pages, tok / T);
-  uint32_t q = 0;
+  uint4 q = make_uint4(0, 0, 0, 0);
   float s = 0.f;
   if (page < 0) {
-    if (p.status && lane == 0) *p.status = DSB_ERR_ARG;
+    if (p.status && c == 0) *p.status = DSB_ERR_ARG;
   } else {
     const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
-    q = reinterpret_cast<const uint32_t*>((which ? p.pool.v : p.pool.k) + (block * T + tok % T) * kD)[lane];
+    q = reinterpret_cast<const uint4*>((which ? p.pool.v : p.pool.k) + (block * T + tok % T) * kD)[c];
     s = pow2i((which ? p.pool.v_exp : p.pool.k_exp)[block]);
   }
-  uint2 o;
-  o.x = pack_bf16x2(e4m3_to_float(q & 255u) * s, e4m3_to_float((q >> 8) & 255u) * s);
-  o.y = pack_bf16x2(e4m3_to_float((q >> 16) & 255u) * s, e4m3_to_float(q >> 24) * s);
-  reinterpret_cast<uint2*>(p.dst[which] + b * p.sb[which] + i * p.sn[which] + h * p.sh[which])[lane] = o;
+  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    o[2 * k] = pack_bf16x2(e4m3_to_float(u[k] & 255u) * s, e4m3_to_float((u[k] >> 8) & 255u) * s);
+    o[2 * k + 1] = pack_bf16x2(e4m3_to_float((u[k] >> 16) & 255u) * s, e4m3_to_float(u[k] >> 24) * s);
+  }
+  uint4* dst = reinterpret_cast<uint4*>(p.dst[which] + b * p.sb[which] + i * p.sn[which] + h * p.sh[which]) + 2 * c;
+  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 // --------------------------------------------------------------------- attention
@@ -182,7 +231,7 @@ constexpr int kAttnStages = 3;
 constexpr int kStageBytes = 2 * kTile * kD;
 constexpr int kAttnRing = kAttnWarps * kAttnStages * kStageBytes;
 constexpr int kAttnDynSmem = kAttnRing + 1024;
-constexpr int kMinShare = 8;    // tiles: fewer are not worth another warp
+constexpr int kMinShare = DSB_KV_UNCUT_TOKENS / kTile;  // tiles: fewer are not worth another warp
 constexpr int kPartRow = 132;   // floats of a partial row: 128 columns, reference exponent, sum, two unused
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -240,10 +289,10 @@ __device__ __forceinline__ int64_t count_tiles(const KvWork& w, int pairs, int64
   }
   return sum * w.heads;
 }
-// tiles per warp
-__host__ __device__ __forceinline__ int64_t share_of(int64_t total, int warps) {
+// tiles per warp, at least `least`
+__device__ __forceinline__ int64_t share_of(int64_t total, int warps, int least) {
   const int64_t s = (total + warps - 1) / warps;
-  return s < kMinShare ? kMinShare : s;
+  return s < least ? least : s;
 }
 
 // A place in the sequence of tiles: a tile of an item, whose rows see `ext` keys.
@@ -302,10 +351,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
     }
   }
   const int64_t total = count_tiles(work, pairs, 0, nullptr, nullptr);
-  const int64_t share = share_of(total, n_warps), first = me * share;
+  const int64_t share = share_of(total, n_warps, parts ? kMinShare : 1);
+  int64_t first = me * share, end = min(first + share, total);
   if (first >= total) return;
-  const int n_mine = static_cast<int>(min(share, total - first));
   KvCursor fetch = find_tile(work, pairs, first);
+  if (!parts) {
+    // nothing is cut: the items that begin in this share, to their ends
+    if (fetch.tile > 0) {
+      first += (fetch.ext + kTile - 1) / kTile - fetch.tile;
+      if (first >= end) return;
+      fetch = find_tile(work, pairs, first);
+    }
+    if (end < total) {
+      const KvCursor last = find_tile(work, pairs, end);
+      if (last.tile > 0) end += (last.ext + kTile - 1) / kTile - last.tile;
+    }
+  }
+  const int n_mine = static_cast<int>(end - first);
   KvCursor at = fetch;
 
   // block (page * heads + head) of the 16 keys from `key` on, or -1
@@ -633,7 +695,7 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(KvAttn p, KvWork work, 
   __shared__ KvCursor item;
   __shared__ int64_t item_share;
   if (threadIdx.x < 32) {
-    const int64_t total = count_tiles(work, pairs, 0, nullptr, nullptr), share = share_of(total, n_warps);
+    const int64_t total = count_tiles(work, pairs, 0, nullptr, nullptr), share = share_of(total, n_warps, kMinShare);
     const int64_t border = (blockIdx.x + 1) * share;
     KvCursor c = {-1, 0, 0, 0};
     if (border < total) {
@@ -739,7 +801,14 @@ extern "C" int dsb_kv_append(const dsb_kv_cache* cache, const void* k, int64_t k
   p.rope_row0 = rope_row0;
   p.status = status;
   const dim3 grid(kv_span_pages(n, T), p.pool.heads, B * 2);
-  const cudaError_t err = launch_kernel(kv_append_kernel, grid, 128, 0, reinterpret_cast<cudaStream_t>(stream), p);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t err;
+  switch (T) {
+    case 16: err = launch_kernel(kv_append_kernel<128, 2>, grid, 128, 0, st, p); break;
+    case 32: err = launch_kernel(kv_append_kernel<128, 4>, grid, 128, 0, st, p); break;
+    case 64: err = launch_kernel(kv_append_kernel<128, 8>, grid, 128, 0, st, p); break;
+    default: err = launch_kernel(kv_append_kernel<256, 8>, grid, 256, 0, st, p); break;
+  }
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }
 
@@ -763,7 +832,9 @@ extern "C" int dsb_kv_read(const dsb_kv_cache* cache, const int32_t* table, int6
   p.first = first;
   p.n = n;
   p.status = status;
-  const dim3 grid((n - 1) / 8 + 1, p.pool.heads, B * 2);
+  const int64_t blocks = (static_cast<int64_t>(n) * p.pool.heads - 1) / 32 + 1;
+  if (blocks > 0x7fffffff) return DSB_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(blocks), 1, B * 2);
   const cudaError_t err = launch_kernel(kv_read_kernel, grid, 256, 0, reinterpret_cast<cudaStream_t>(stream), p);
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }
@@ -819,9 +890,6 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   p.status = status;
   const int64_t rows = static_cast<int64_t>(Sq) * p.G, row_tiles = (rows - 1) / kRowTile + 1, pairs = row_tiles * B;
   if (rows > 0x7fffff00 || pairs > 0x7fffffff) return DSB_ERR_UNSUPPORTED;
-  const int warps = attn_warps();
-  if (warps <= 0) return DSB_ERR_CUDA;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < dsb_kv_attn_workspace_bytes()) return DSB_ERR_ARG;
   KvWork w = {};
   w.Sq = Sq;
   w.G = p.G;
@@ -832,25 +900,31 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   w.capacity = p.tab.capacity(p.pool.T);
   w.lens = lens;
   w.len_all = len_all;
+  // Short sequences (at most kMinShare tiles): whole items for each warp, nothing to combine.  No more CTAs than the longest
+  // possible lengths need.
+  const int64_t most_len = lens ? w.capacity : len_all, item_tiles = (most_len + kTile - 1) / kTile;
+  const int64_t items = pairs * p.pool.heads;
+  const bool cut = item_tiles > kMinShare;
+  if (cut && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))) return DSB_ERR_ARG;
+  const int warps = attn_warps();
+  if (warps <= 0) return DSB_ERR_CUDA;
+  if (cut && workspace_bytes < dsb_kv_attn_workspace_bytes()) return DSB_ERR_ARG;
+  int64_t ctas = cut ? (items * item_tiles + kMinShare * kAttnWarps - 1) / (kMinShare * kAttnWarps) : (items + kAttnWarps - 1) / kAttnWarps;
+  if (ctas < 1) ctas = 1;
+  if (ctas > warps / kAttnWarps) ctas = warps / kAttnWarps;
   const uint64_t map_rows = static_cast<uint64_t>(p.pool.n_pages) * p.pool.heads * p.pool.T;
   CUtensorMap mk, mv;
   const uint32_t box = p.pool.T == 16 ? 16 : 32;
   if ((rc = make_tmap_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.pool.k, map_rows, kD, kD, box, kD)) != DSB_OK) return rc;
   if ((rc = make_tmap_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.pool.v, map_rows, kD, kD, box, kD)) != DSB_OK) return rc;
-  // no more CTAs than the longest possible lengths need
-  const int64_t most_len = lens ? w.capacity : len_all;
-  const int64_t tiles = pairs * p.pool.heads * ((most_len + kTile - 1) / kTile);
-  int64_t ctas = (tiles + kMinShare * kAttnWarps - 1) / (kMinShare * kAttnWarps);
-  if (ctas < 1) ctas = 1;
-  if (ctas > warps / kAttnWarps) ctas = warps / kAttnWarps;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int n_pairs = static_cast<int>(pairs);
-  float* parts = reinterpret_cast<float*>(workspace);
+  float* parts = cut ? reinterpret_cast<float*>(workspace) : nullptr;
   cudaError_t err = launch_kernel(p.pool.T == 16 ? kv_attn_kernel<true> : kv_attn_kernel<false>, static_cast<unsigned>(ctas),
                                   kAttnWarps * 32, kAttnDynSmem, st, mk, mv, p, w, n_pairs, parts);
   if (err != cudaSuccess) return DSB_ERR_CUDA;
   const int n_warps = static_cast<int>(ctas) * kAttnWarps;
-  if (tiles > kMinShare && n_warps > 1)
+  if (cut && n_warps > 1)
     err = launch_kernel(kv_combine_kernel, n_warps - 1, 256, 0, st, p, w, n_pairs, n_warps, static_cast<const float*>(parts));
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }

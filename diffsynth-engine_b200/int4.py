@@ -2,8 +2,8 @@
 ``c`` (0..15) stands for ``s * (c - 8)``, or ``s * c + m``.  GGUF Q4_0, Q4_1 and Q4_K weights are taken over with their own
 codes; any other weight is quantised here.  A few activation rows are multiplied as they are (``dsb_gemv_int4``); for more rows
 the weight is expanded to bf16 (``dequant``) and goes through the GEMM."""
-from dataclasses import dataclass
-from typing import List, Optional
+import ctypes
+from typing import List
 
 import torch
 
@@ -16,30 +16,36 @@ MAX_ROWS = 32     # DSB_INT4_MAX_ROWS: activation rows of one product
 GGUF_TYPES = ("Q4_0", "Q4_1", "Q4_K")
 
 
-@dataclass
 class Int4Weight:
-    """A 4-bit ``[N, K]`` weight laid out for the kernels (``dsb_int4_pack``)."""
-    payload: torch.Tensor            # uint8 [ceil(N/16), ceil(K/64), 512]
-    scales: torch.Tensor             # fp16 [ceil(N/16), tiles, 8, groups per tile, 2]
-    mins: Optional[torch.Tensor]     # the same shape, or None
-    N: int
-    K: int
-    group: int
+    """A 4-bit ``[N, K]`` weight laid out for the kernels (``dsb_int4_pack``): ``payload`` uint8 ``[ceil(N/16), ceil(K/64), 512]``,
+    ``scales`` and ``mins`` (or None) fp16 ``[ceil(N/16), tiles, 8, groups per tile, 2]``.  The tensors cannot be replaced: the
+    kernels take their addresses, which are checked here."""
 
-    @property
-    def out_features(self):
-        return self.N
+    __slots__ = ("_t", "N", "K", "group", "_device", "_args", "_ref")
 
-    @property
-    def in_features(self):
-        return self.K
+    def __init__(self, payload, scales, mins, N: int, K: int, group: int):
+        if N <= 0 or K <= 0 or K % 2 or group not in GROUPS:
+            raise _lib.DsbError(f"Int4Weight: [{N}, {K}] in groups of {group} is no 4-bit weight")
+        rb, tiles = -(-N // 16), -(-K // (128 if group == 128 else 64))
+        need = rb * tiles * 16 * (2 if group == 32 else 1)
+        if payload.dtype != torch.uint8 or not payload.is_contiguous() or payload.numel() != rb * -(-K // 64) * 512:
+            raise _lib.DsbError("Int4Weight: the payload is not a contiguous uint8 tensor of its size")
+        for t in (scales, mins):
+            if t is not None and (t.dtype != torch.float16 or not t.is_contiguous() or t.numel() != need or t.device != payload.device):
+                raise _lib.DsbError("Int4Weight: scales and mins are contiguous float16 tensors of their size, where the payload is")
+        self._t, self.N, self.K, self.group, self._device = (payload, scales, mins), N, K, group, payload.get_device()
+        self._args = _lib.Int4Args(payload.data_ptr(), scales.data_ptr(), _ptr(mins), N, K, group)
+        self._ref = ctypes.byref(self._args)
 
-    @property
-    def device(self):
-        return self.payload.device
+    payload = property(lambda self: self._t[0])
+    scales = property(lambda self: self._t[1])
+    mins = property(lambda self: self._t[2])
+    out_features = property(lambda self: self.N)
+    in_features = property(lambda self: self.K)
+    device = property(lambda self: self._t[0].device)
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.payload, self.scales, self.mins) if t is not None)
+        return sum(t.numel() * t.element_size() for t in self._t if t is not None)
 
 
 def _empty(N, K, group, has_min, device) -> Int4Weight:
@@ -50,19 +56,11 @@ def _empty(N, K, group, has_min, device) -> Int4Weight:
                       torch.empty_like(scales) if has_min else None, N, K, group)
 
 
-def _check_weight(w: Int4Weight):
-    """The kernels take raw pointers: what they rely on is checked here."""
-    if not isinstance(w, Int4Weight):
+def _check_weight(w):
+    if type(w) is not Int4Weight:
         raise _lib.DsbError("expected an Int4Weight (int4.from_codes, int4.quantize, int4.from_gguf)")
-    if w.N <= 0 or w.K <= 0 or w.K % 2 or w.group not in GROUPS:
-        raise _lib.DsbError(f"Int4Weight: [{w.N}, {w.K}] in groups of {w.group} is no 4-bit weight")
-    rb, tiles = -(-w.N // 16), -(-w.K // (128 if w.group == 128 else 64))
-    need = rb * tiles * 16 * (2 if w.group == 32 else 1)
-    if w.payload.dtype != torch.uint8 or not w.payload.is_contiguous() or w.payload.numel() != rb * -(-w.K // 64) * 512:
-        raise _lib.DsbError("Int4Weight: the payload is not a contiguous uint8 tensor of its size")
-    for t in (w.scales, w.mins):
-        if t is not None and (t.dtype != torch.float16 or not t.is_contiguous() or t.numel() != need):
-            raise _lib.DsbError("Int4Weight: scales and mins are contiguous float16 tensors of their size")
+    if w._device != torch._C._cuda_getDevice():
+        _require_cuda(w.payload)
 
 
 def from_codes(codes, scales, mins=None, group=32) -> Int4Weight:
@@ -153,13 +151,12 @@ def stack(parts: List[Int4Weight]) -> Int4Weight:
 def dequant(w: Int4Weight, out=None):
     """The weight as bf16 ``[N, K]``."""
     _check_weight(w)
-    _require_cuda(w.payload, w.scales, w.mins, out)
+    _require_cuda(out)
     if out is None:
         out = torch.empty((w.N, w.K), dtype=torch.bfloat16, device=w.device)
     if out.dtype != torch.bfloat16 or tuple(out.shape) != (w.N, w.K) or out.stride(1) != 1 or (w.N > 1 and out.stride(0) < w.K):
         raise _lib.DsbError(f"int4.dequant output must be bfloat16 [{w.N}, {w.K}] rows")
-    rc = _lib.lib().dsb_int4_dequant(_ptr(w.payload), _ptr(w.scales), _ptr(w.mins), w.N, w.K, w.group, _ptr(out),
-                                     max(out.stride(0), w.K), _stream())
+    rc = _lib.lib().dsb_int4_dequant(w._ref, _ptr(out), max(out.stride(0), w.K), _stream())
     check(rc, "dsb_int4_dequant")
     return out
 
@@ -168,29 +165,30 @@ def gemv(w: Int4Weight, x, bias=None, act_in=ACT_NONE, act_out=ACT_NONE, out=Non
     """``act_out(act_in(x) @ w.T + bias)`` for one row ``x[K]`` or up to ``MAX_ROWS`` rows ``x[M, K]`` (float32 or bfloat16),
     fp32 arithmetic; ``out`` (default: the dtype of ``x``) is float32 or bfloat16 and, with ``accumulate``, added to."""
     _check_weight(w)
-    _require_cuda(w.payload, w.scales, w.mins, x, bias, out)
-    rows = x if x.dim() == 2 else x.unsqueeze(0)
-    if rows.dim() != 2 or rows.shape[1] != w.K or (rows.stride(1) != 1 and rows.shape[1] > 1):
-        raise _lib.DsbError(f"int4.gemv takes x as [{w.K}] or [M, {w.K}] with contiguous rows, got {tuple(x.shape)}")
-    M = rows.shape[0]
+    _require_cuda(x, bias, out)
+    N, K = w.N, w.K
+    one = x.dim() == 1
+    M, ld_x = (1, K) if one else (x.shape[0], x.stride(0))
+    if x.dim() > 2 or x.shape[-1] != K or x.stride(-1) != 1 or (M > 1 and ld_x < K):
+        raise _lib.DsbError(f"int4.gemv takes x as [{K}] or [M, {K}] with contiguous rows that do not overlap, got {tuple(x.shape)}")
     if M > MAX_ROWS:
         raise _lib.DsbError(f"int4.gemv takes up to {MAX_ROWS} rows, got {M}: expand the weight (int4.dequant) for more")
+    x_bf16 = x.dtype == torch.bfloat16
+    if not x_bf16 and x.dtype != torch.float32:
+        raise _lib.DsbError(f"int4.gemv takes float32 or bfloat16 rows, got {x.dtype}")
     if out is None:
         if accumulate:
             raise _lib.DsbError("int4.gemv: accumulate needs an out to add to")
-        out = torch.empty((M, w.N) if x.dim() == 2 else (w.N,), dtype=x.dtype, device=x.device)
-    o = out if out.dim() == 2 else out.unsqueeze(0)
-    if o.dim() != 2 or tuple(o.shape) != (M, w.N) or (o.stride(1) != 1 and w.N > 1):
-        raise _lib.DsbError(f"int4.gemv output must be [{M}, {w.N}] with contiguous rows, got {tuple(out.shape)}")
-    for t in (rows, o):
-        if t.dtype != torch.bfloat16 and t.dtype != torch.float32:
-            raise _lib.DsbError(f"int4.gemv takes float32 or bfloat16 rows, got {t.dtype}")
-        if M > 1 and t.stride(0) < t.shape[1]:
-            raise _lib.DsbError("int4.gemv rows must not overlap")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != w.N or not bias.is_contiguous()):
-        raise _lib.DsbError(f"int4.gemv bias must be contiguous float32 with {w.N} elements")
-    rc = _lib.lib().dsb_gemv_int4(_ptr(w.payload), _ptr(w.scales), _ptr(w.mins), w.N, w.K, w.group, _ptr(rows), rows.stride(0),
-                                  rows.dtype == torch.bfloat16, _ptr(bias), _ptr(o), o.stride(0), o.dtype == torch.bfloat16, M, act_in,
-                                  act_out, 1 if accumulate else 0, _stream())
+        out, ld_y, y_bf16 = torch.empty((N,) if one else (M, N), dtype=x.dtype, device=x.device), N, x_bf16
+    else:
+        ld_y, y_bf16 = N if out.dim() == 1 else out.stride(0), out.dtype == torch.bfloat16
+        if out.dim() != x.dim() or tuple(out.shape) != ((N,) if one else (M, N)) or (out.stride(-1) != 1 and N > 1) or (M > 1 and ld_y < N):
+            raise _lib.DsbError(f"int4.gemv output must be {(N,) if one else (M, N)} with contiguous rows, got {tuple(out.shape)}")
+        if not y_bf16 and out.dtype != torch.float32:
+            raise _lib.DsbError(f"int4.gemv writes float32 or bfloat16 rows, got {out.dtype}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
+        raise _lib.DsbError(f"int4.gemv bias must be contiguous float32 with {N} elements")
+    rc = _lib.lib().dsb_gemv_int4(w._ref, x.data_ptr(), ld_x, x_bf16, _ptr(bias), out.data_ptr(), ld_y, y_bf16, M, act_in, act_out,
+                                  accumulate, _stream())
     check(rc, "dsb_gemv_int4")
     return out

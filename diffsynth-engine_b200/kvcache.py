@@ -11,6 +11,10 @@ from ._lib import check
 from .ops import _ptr, _require_cuda, _stream, status_word
 
 HEAD_DIM = 128
+_SM_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+UNCUT_TOKENS = 256     # sequences up to this length are never cut (DSB_KV_UNCUT_TOKENS): no workspace
+# Queries from which on a length that the caller knows is worth bf16 rows of the whole sequence and the dense attention kernel
+DENSE_QUERIES = 256
 PAGE_TOKENS = (16, 32, 64, 128)
 
 
@@ -37,6 +41,8 @@ class PagedKVCache:
         self._t = (k, v, k_exp, v_exp)
         self._args = _lib.KVCacheArgs(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), *k.shape[:3])
         self._ref = ctypes.byref(self._args)
+        self._device = k.get_device()
+        self.pages, self.heads, self.page_tokens = k.shape[:3]
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_tokens: int = 64, device="cuda") -> "PagedKVCache":
@@ -48,32 +54,45 @@ class PagedKVCache:
     v = property(lambda self: self._t[1])
     k_exp = property(lambda self: self._t[2])
     v_exp = property(lambda self: self._t[3])
-    pages = property(lambda self: self._args.n_pages)
-    heads = property(lambda self: self._args.heads)
-    page_tokens = property(lambda self: self._args.page_tokens)
 
     def pages_for(self, tokens: int) -> int:
         """Table entries that a sequence of ``tokens`` needs."""
         return -(-tokens // self.page_tokens)
 
 
+def _here(cache, *ts):
+    """The current device, on which the cache and every tensor of a call must live."""
+    dev = cache._device
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        _require_cuda(cache.k)
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _require_cuda(t)
+    return dev
+
+
 def _table(table, B):
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or table.shape[1] == 0 or table.stride(1) != 1 \
-            or (B > 1 and table.stride(0) < table.shape[1]):
+    if table.dtype != torch.int32 or table.dim() != 2:
         raise _lib.DsbError(f"the page table is an int32 [{B}, pages] tensor with contiguous rows")
-    return max(table.stride(0), table.shape[1]), table.shape[1]
+    (rows, width), (ld, inner) = table.shape, table.stride()
+    if rows != B or width == 0 or (inner != 1 and width > 1) or (ld < width and B > 1):
+        raise _lib.DsbError(f"the page table is an int32 [{B}, pages] tensor with contiguous rows")
+    return (ld if ld > width else width), width
 
 
 def _per_sequence(t, B, what):
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or not t.is_contiguous():
         raise _lib.DsbError(f"{what} is an int or a contiguous int32 [{B}] tensor")
 
 
 def _rows4(t, what):
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or t.stride(3) != 1 or t.data_ptr() % 16 \
-            or any(s % 8 or s < 0 for s in t.stride()[:3]):
+    """(shape, strides, address) of rows that the kernels take."""
+    shape, st, ptr = t.shape, t.stride(), t.data_ptr()
+    if len(shape) != 4 or shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or st[3] != 1 or ptr % 16 \
+            or (st[0] | st[1] | st[2]) & 7 or st[0] < 0 or st[1] < 0 or st[2] < 0:
         raise _lib.DsbError(f"{what} is a bf16 [B, tokens, heads, 128] tensor with a contiguous head dimension, 16-byte aligned, "
                             "with strides that are multiples of 8")
+    return shape, st, ptr
 
 
 def append(cache: PagedKVCache, k, v, table, start, counts=None, rope=None, rope_row0: int = 0):
@@ -81,42 +100,49 @@ def append(cache: PagedKVCache, k, v, table, start, counts=None, rope=None, rope
     (int32 ``[B, pages]``), from position ``start`` (int, or int32 ``[B]``) on; ``counts`` (int32 ``[B]``): how many of the n rows
     belong to each sequence.  ``rope`` (fp32 ``[rows, 64, 2]`` = cos, sin): ``k`` is rotated by row ``rope_row0 + position``.
     A position or page outside its table leaves that part unwritten and raises at the next ``ops.check_status``."""
-    B, n = k.shape[0], k.shape[1]
     dev_start = start if isinstance(start, torch.Tensor) else None
-    _require_cuda(cache.k, k, v, table, dev_start, counts, rope)
-    _rows4(k, "k")
-    _rows4(v, "v")
-    if v.shape != k.shape or k.shape[2] != cache.heads:
+    dev = _here(cache, k, v, table, dev_start, counts, rope)
+    shape, ks, k_ptr = _rows4(k, "k")
+    v_shape, vs, v_ptr = _rows4(v, "v")
+    B, n, heads, _ = shape
+    if v_shape != shape or heads != cache.heads:
         raise _lib.DsbError(f"k and v are [B, n, {cache.heads}, 128] rows of one shape")
     ld, width = _table(table, B)
     if dev_start is not None:
         _per_sequence(dev_start, B, "start")
+        start = 0
     elif not 0 <= start <= width * cache.page_tokens - (n if counts is None else 0):
         raise _lib.DsbError(f"{n} rows from position {start} on do not fit a table of {width} pages")
     if counts is not None:
         _per_sequence(counts, B, "counts")
+    rope_rows = 0
     if rope is not None:
-        if rope.dtype != torch.float32 or rope.dim() != 3 or tuple(rope.shape[1:]) != (64, 2) or not rope.is_contiguous():
+        if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (64, 2) or not rope.is_contiguous():
             raise _lib.DsbError("rope is a contiguous float32 [rows, 64, 2] table")
         if rope.data_ptr() % 16 or not -(1 << 31) <= rope_row0 < 1 << 31:
             raise _lib.DsbError("rope is 16-byte aligned and rope_row0 a 32-bit number")
-    rc = _lib.lib().dsb_kv_append(
-        cache._ref, _ptr(k), k.stride(0), k.stride(1), k.stride(2), _ptr(v), v.stride(0), v.stride(1), v.stride(2), B, n,
-        _ptr(table), ld, width, _ptr(dev_start), 0 if dev_start is not None else start, _ptr(counts), _ptr(rope),
-        0 if rope is None else rope.shape[0], rope_row0, _ptr(status_word(k.device)), _stream())
+        rope_rows = rope.shape[0]
+    rc = _lib.lib().dsb_kv_append(cache._ref, k_ptr, ks[0], ks[1], ks[2], v_ptr, vs[0], vs[1], vs[2], B, n, table.data_ptr(), ld, width,
+                                  _ptr(dev_start), start, _ptr(counts), _ptr(rope), rope_rows, rope_row0, _status_ptr(dev), _stream())
     check(rc, "dsb_kv_append")
+
+
+def _status_ptr(dev: int):
+    word = ops._status.get(dev)
+    return (word if word is not None else status_word(torch.device("cuda", dev))).data_ptr()
 
 
 def read(cache: PagedKVCache, table, n: int, first: int = 0):
     """Tokens ``first .. first + n - 1`` of each sequence as bf16 ``(k, v)``, each ``[B, n, heads, 128]`` (exact)."""
-    _require_cuda(cache.k, table)
+    dev = _here(cache, table)
     B = table.shape[0]
     ld, width = _table(table, B)
     if n < 0 or first < 0 or first + n > width * cache.page_tokens:
         raise _lib.DsbError(f"tokens {first}..{first + n - 1} are not in a table of {width} pages")
-    k, v = (torch.empty((B, n, cache.heads, HEAD_DIM), dtype=torch.bfloat16, device=table.device) for _ in range(2))
-    rc = _lib.lib().dsb_kv_read(cache._ref, _ptr(table), ld, width, B, first, n, _ptr(k), k.stride(0), k.stride(1), k.stride(2),
-                                _ptr(v), v.stride(0), v.stride(1), v.stride(2), _ptr(status_word(table.device)), _stream())
+    k, v = torch.empty((2, B, n, cache.heads, HEAD_DIM), dtype=torch.bfloat16, device=table.device).unbind(0)
+    sb, sn, sh, _ = k.stride()
+    rc = _lib.lib().dsb_kv_read(cache._ref, table.data_ptr(), ld, width, B, first, n, k.data_ptr(), sb, sn, sh, v.data_ptr(), sb, sn, sh,
+                                _status_ptr(dev), _stream())
     check(rc, "dsb_kv_read")
     return k, v
 
@@ -124,15 +150,15 @@ def read(cache: PagedKVCache, table, n: int, first: int = 0):
 _workspace = {}
 
 
-def workspace_bytes(device) -> int:
-    """Bytes of scratch that a call of :func:`attend` on ``device`` takes (``dsb_kv_attn_workspace_bytes``)."""
-    n = _workspace.get(device.index)
+def workspace_bytes(device: int) -> int:
+    """Bytes of scratch that a call of :func:`attend` on a device takes (``dsb_kv_attn_workspace_bytes``)."""
+    n = _workspace.get(device)
     if n is None:
         with torch.cuda.device(device):
-            n = _workspace[device.index] = int(_lib.lib().dsb_kv_attn_workspace_bytes())
+            n = int(_lib.lib().dsb_kv_attn_workspace_bytes())
         if n <= 0:
-            _workspace.pop(device.index)
             raise _lib.DsbError("dsb_kv_attn_workspace_bytes failed")
+        _workspace[device] = n
     return n
 
 
@@ -142,28 +168,43 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     position ``lens - Sq + i`` (the queries are the sequence's last tokens, already appended).  A query that sees no key gives
     zeros."""
     dev_lens = lens if isinstance(lens, torch.Tensor) else None
-    _require_cuda(q, cache.k, table, dev_lens, out)
-    _rows4(q, "q")
-    B, Sq, H, _ = q.shape
-    if H == 0 or H % cache.heads:
-        raise _lib.DsbError(f"{H} query heads do not share {cache.heads} cache heads evenly")
+    dev = _here(cache, q, table, dev_lens, out)
+    shape, qs, q_ptr = _rows4(q, "q")
+    B, Sq, H, _ = shape
+    heads = cache.heads
+    if H == 0 or H % heads:
+        raise _lib.DsbError(f"{H} query heads do not share {heads} cache heads evenly")
     ld, width = _table(table, B)
+    most = width * cache.page_tokens
     if dev_lens is not None:
         _per_sequence(dev_lens, B, "lens")
-    elif not 0 <= lens <= width * cache.page_tokens:
+        lens = 0
+    elif not 0 <= lens <= most:
         raise _lib.DsbError(f"{lens} tokens do not fit a table of {width} pages")
-    if out is None:
-        out = torch.empty((B, Sq, H, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     else:
-        _rows4(out, "out")
-        if out.shape != q.shape or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        most = lens
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        out_ptr, os = out.data_ptr(), out.stride()
+    else:
+        out_shape, os, out_ptr = _rows4(out, "out")
+        if out_shape != shape or any(st == 0 and n > 1 for st, n in zip(os, shape)):
             raise _lib.DsbError("out has the shape of q and a place for each of its values")
     if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(HEAD_DIM)
-    ws = torch.empty(workspace_bytes(q.device), dtype=torch.uint8, device=q.device)
+        sm_scale = _SM_SCALE
+    if dev_lens is None and not causal and Sq >= DENSE_QUERIES and lens > 0 and B > 0:
+        k, v = read(cache, table, lens)
+        share = H // heads
+        for g in range(share):      # a cache head's queries, one of its query heads at a time
+            ops.flash_attn(q[:, :, g::share], k, v, out=out[:, :, g::share], sm_scale=sm_scale)
+        return out
+    ws_ptr = ws_bytes = 0
+    if most > UNCUT_TOKENS:         # a sequence may be cut along its keys
+        ws_bytes = workspace_bytes(dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        ws_ptr = ws.data_ptr()
     rc = _lib.lib().dsb_kv_attn(
-        cache._ref, _ptr(q), q.stride(0), q.stride(1), q.stride(2), _ptr(out), out.stride(0), out.stride(1), out.stride(2), B, Sq, H,
-        _ptr(table), ld, width, _ptr(dev_lens), 0 if dev_lens is not None else lens, 1 if causal else 0, float(sm_scale),
-        _ptr(ws), ws.numel(), _ptr(status_word(q.device)), _stream())
+        cache._ref, q_ptr, qs[0], qs[1], qs[2], out_ptr, os[0], os[1], os[2], B, Sq, H, table.data_ptr(), ld, width, _ptr(dev_lens), lens,
+        1 if causal else 0, sm_scale, ws_ptr, ws_bytes, _status_ptr(dev), _stream())
     check(rc, "dsb_kv_attn")
     return out

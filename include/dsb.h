@@ -420,9 +420,15 @@ int dsb_int4_from_gguf(int qtype, const uint8_t* raw, int64_t row_bytes, int N, 
 int dsb_int4_pack(const uint8_t* codes, int64_t ld_codes, const void* scales, const void* mins, int64_t ld_scales, int N, int K,
                   int group, void* payload, void* out_scales, void* out_mins, void* stream);
 
+typedef struct {
+  const void* payload;
+  const void* scales;
+  const void* mins; /* or NULL */
+  int N, K, group;
+} dsb_int4_weight;
+
 /* The laid-out weight as bf16 [N, ld_out]: the fp32 value s * (c - 8) or s * c + m, rounded. */
-int dsb_int4_dequant(const void* payload, const void* scales, const void* mins, int N, int K, int group, void* out, int64_t ld_out,
-                     void* stream);
+int dsb_int4_dequant(const dsb_int4_weight* w, void* out, int64_t ld_out, void* stream);
 
 /*
  * y = act_out(W . act_in(x) + bias) (+ y before, with `accumulate`) for M <= DSB_INT4_MAX_ROWS rows x[M, ld_x] (fp32 or bf16; any
@@ -430,9 +436,8 @@ int dsb_int4_dequant(const void* payload, const void* scales, const void* mins, 
  * not overlap x.
  */
 #define DSB_INT4_MAX_ROWS 32
-int dsb_gemv_int4(const void* payload, const void* scales, const void* mins, int N, int K, int group, const void* x, int64_t ld_x,
-                  int x_bf16, const float* bias, void* y, int64_t ld_y, int y_bf16, int M, int act_in, int act_out, int accumulate,
-                  void* stream);
+int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld_x, int x_bf16, const float* bias, void* y, int64_t ld_y,
+                  int y_bf16, int M, int act_in, int act_out, int accumulate, void* stream);
 
 /*
  * Paged 8-bit cache of keys and values: k and v are e4m3 [n_pages, heads, page_tokens, 128] (contiguous, 128-byte aligned), k_exp
@@ -474,9 +479,11 @@ int dsb_kv_read(const dsb_kv_cache* cache, const int32_t* table, int64_t ld_tabl
  * o = softmax(q . k^T * sm_scale) . v of q [B, Sq, H, 128] over the first lens[b] (lens NULL: len_all) tokens of each sequence;
  * query head h reads cache head h / (H / heads).  causal: query i sees the keys up to position lens[b] - Sq + i.  A query that
  * sees no key gives zeros.  workspace: dsb_kv_attn_workspace_bytes() bytes, 16-byte aligned, for the partial results of sequences
- * that are cut along their keys; calls that may run at the same time need one each.
+ * that are cut along their keys; calls that may run at the same time need one each.  NULL will do where no sequence can be longer
+ * than DSB_KV_UNCUT_TOKENS (len_all, or width * page_tokens with lens): those are never cut.
  * Stands beside dsb_flash_attn (models/wan/wan_dit.py:18-22,143-149), whose keys and values are bf16 rows.
  */
+#define DSB_KV_UNCUT_TOKENS 256
 int64_t dsb_kv_attn_workspace_bytes(void);
 int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_s, int64_t q_stride_h, void* o,
                 int64_t o_stride_b, int64_t o_stride_s, int64_t o_stride_h, int B, int Sq, int H, const int32_t* table,

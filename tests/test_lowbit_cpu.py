@@ -91,7 +91,8 @@ def test_c_entries_refuse_before_any_launch(dsb):
     def gemv(**kw):
         a = dict(p=P, s=P, m=None, N=16, K=64, group=32, x=P, ld_x=64, xb=0, bias=None, y=P, ld_y=16, yb=0, M=1, ai=0, ao=0, acc=0)
         a.update(kw)
-        return lib.dsb_gemv_int4(*a.values(), None)
+        a = list(a.values())
+        return lib.dsb_gemv_int4(ctypes.byref(dsb._lib.Int4Args(*a[:6])), *a[6:], None)
 
     for kw in (dict(p=None), dict(s=None), dict(x=None), dict(y=None), dict(N=0), dict(K=0), dict(K=63), dict(group=16), dict(M=33), dict(M=-1), dict(ai=1),
                dict(ao=4), dict(ao=-1), dict(p=P + 8), dict(s=P + 4), dict(x=P + 2), dict(M=2, ld_x=63), dict(M=2, ld_y=15), dict(y=P + 2)):
@@ -104,7 +105,8 @@ def test_c_entries_refuse_before_any_launch(dsb):
     assert lib.dsb_int4_from_gguf(3, P, 20, 1, 32, P, 16, P, None, None) == ARG       # Q4_1 has
     assert lib.dsb_int4_from_gguf(12, P, 143, 1, 256, P, 128, P, P, None) == ARG
     assert lib.dsb_int4_quantize(P, 63, 0, 1, 64, 32, P, 32, P, None, None) == ARG
-    assert lib.dsb_int4_dequant(P, P, None, 16, 64, 32, P, 63, None) == ARG
+    assert lib.dsb_int4_dequant(ctypes.byref(dsb._lib.Int4Args(P, P, None, 16, 64, 32)), P, 63, None) == ARG
+    assert lib.dsb_gemv_int4(None, P, 64, 0, None, P, 16, 0, 1, 0, 0, 0, None) == ARG and lib.dsb_int4_dequant(None, P, 64, None) == ARG
 
     def cache(**kw):
         a = dict(k=P, v=P, k_exp=P, v_exp=P, n_pages=4, heads=2, page_tokens=16)
@@ -118,7 +120,7 @@ def test_c_entries_refuse_before_any_launch(dsb):
         return lib.dsb_kv_attn(c or cache(), *a.values(), None)
 
     for kw in (dict(q=None), dict(o=P + 8), dict(H=3), dict(H=0), dict(B=-1), dict(Sq=-1), dict(table=None), dict(width=0), dict(ld=1), dict(len_all=33),
-               dict(len_all=-1), dict(qs=4), dict(oh=-8)):
+               dict(len_all=-1), dict(qs=4), dict(oh=-8), dict(len_all=300, width=32, ld=32)):
         assert attn(**kw) == ARG, kw
     for c in (cache(k=None), cache(v_exp=None), cache(n_pages=0), cache(heads=0), cache(v=P + 16)):
         assert attn(c) == ARG

@@ -36,8 +36,7 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
-// 2^e for e in [-128, 127)
-__device__ __forceinline__ float pow2i(int e) { return e < -126 ? ldexpf(1.f, e) : __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // ------------------------------------------------------------------------ append
 struct KvAppend {
@@ -136,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(KvAppend p) {
   if (s.slot > 0) {
     e = max(e, was);
     if (e > was) {
-      const float fall = pow2i(was - e);
+      const float fall = pow2i(max(was - e, -126));   // (2^-127 and 2^-128 too take every e4m3 value to zero)
       for (int i = tid; i < s.slot * (kD / 4); i += THREADS) {
         uint32_t* at = reinterpret_cast<uint32_t*>(dst) + i;
         const uint32_t q = *at;
@@ -222,16 +221,20 @@ struct KvAttn {
 // Per warp: a ring of K and V tiles (TMA, 128-byte swizzle); S = Q K^T and O += P V with 16-bit tensor-core products and fp32
 // sums, fragments taken straight from the e4m3 bytes (exact in fp16).  Q is bf16 times a power of two per row, so exact in fp16
 // too but for values 2^-27 below the row's largest.  The scales: key j's score is t = S * c * 2^(ek + eq) + ev, in powers of two,
-// so that p = 2^(t - m) <= 1 carries the value block's scale, and the row sum adds p * 2^-ev.  p is rounded to fp16: 11 bits,
-// three more than bf16 would keep.
+// so that p = 2^(t - m) carries the value block's scale, and the row sum adds p * 2^-ev.  p is rounded to fp16: 11 bits, three
+// more than bf16 would keep.  The reference m of a row moves only when a score is 2^kSlack above it (p stays below 2^kSlack,
+// and fp16 has room to 2^16): moving it with every new maximum cost a rescaling of O in about every second tile.
 constexpr int kTile = 32;       // keys
 constexpr int kRowTile = 16;
-constexpr int kAttnWarps = 4;   // per CTA; they share nothing
-constexpr int kAttnStages = 3;
+constexpr int kAttnWarps = 4;   // consumers per CTA
+constexpr int kAttnThreads = kAttnWarps * 32 + 32;
+constexpr int kInfoRing = 32;   // tiles whose description is kept: four rounds of the producer
+constexpr int kAttnStages = 3;  // per warp of the stream
 constexpr int kStageBytes = 2 * kTile * kD;
 constexpr int kAttnRing = kAttnWarps * kAttnStages * kStageBytes;
 constexpr int kAttnDynSmem = kAttnRing + 1024;
 constexpr int kMinShare = DSB_KV_UNCUT_TOKENS / kTile;  // tiles: fewer are not worth another warp
+constexpr float kSlack = 8.f;
 constexpr int kPartRow = 132;   // floats of a partial row: 128 columns, reference exponent, sum, two unused
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -248,241 +251,312 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The work of a call: pairs (sequence, row tile), each with the same number of tiles for every cache head.
+// x / d for x * d < 2^46 (the host sees to it): mul is above 2^46 / d by less than 1, so x * mul / 2^46 is above x / d by less
+// than 1 / d.
+struct FastDiv {
+  uint64_t mul;
+  __host__ static FastDiv of(int d) { return {((1ull << 46) + d - 1) / d}; }
+  __device__ __forceinline__ int operator()(int x) const { return static_cast<int>(__umul64hi(static_cast<uint64_t>(x) << 18, mul)); }
+};
+// The work of a call: pairs (sequence, row tile), each with the same number of tiles for every cache head.  (The host keeps the
+// number of all tiles below 2^31.)
 struct KvWork {
-  int Sq, G, heads, T, causal, row_tiles;
+  FastDiv by_G, by_row_tiles, by_heads;
+  int Sq, G, heads, T, shift, causal, rows_tile, row_tiles, pairs;   // T = 1 << shift; rows_tile: rows of an item, 16 per warp
   int64_t capacity;
   const int32_t* lens;
   int len_all;
   __device__ __forceinline__ int length(int b) const { return kv_length(lens ? lens[b] : len_all, capacity); }
   // keys that the last row of a row tile sees
   __device__ __forceinline__ int extent(int len, int rt) const {
-    const int last = min(rt * kRowTile + kRowTile, Sq * G) - 1;
-    return kv_visible(len, Sq, last / G, causal);
+    if (!causal) return len;
+    return kv_visible(len, Sq, by_G(min(rt * rows_tile + rows_tile, Sq * G) - 1), causal);
   }
-  __device__ __forceinline__ int extent_of(int pair) const { return extent(length(pair / row_tiles), pair % row_tiles); }
-  __device__ __forceinline__ int tiles(int pair) const { return (extent_of(pair) + kTile - 1) / kTile; }
+  __device__ __forceinline__ int extent_of(int pair) const {
+    const int b = by_row_tiles(pair);
+    return extent(length(b), pair - b * row_tiles);
+  }
 };
-// Sum of the tiles of all pairs before `limit`, for one cache head; with `find`, the last pair whose tiles begin at or before
-// that many (times heads) tiles.  All lanes of a warp.
-__device__ __forceinline__ int64_t count_tiles(const KvWork& w, int pairs, int64_t find, int* found, int64_t* before) {
-  const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
-  for (int base = 0; base < pairs; base += 32) {
-    const int pair = base + lane;
-    int64_t n = pair < pairs ? w.tiles(pair) : 0, run = n;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-    }
-    if (found) {
-      const bool mine = n > 0 && (sum + run - n) * w.heads <= find && (sum + run) * w.heads > find;
-      const uint32_t vote = __ballot_sync(0xffffffffu, mine);
-      if (vote) {
-        const int src = __ffs(vote) - 1;
-        *found = base + src;
-        *before = __shfl_sync(0xffffffffu, sum + run - n, src) * w.heads;
-      }
-    }
-    sum += __shfl_sync(0xffffffffu, run, 31);
-  }
-  return sum * w.heads;
+__device__ __forceinline__ int tiles_of(int ext) { return (ext + kTile - 1) / kTile; }
+// Tiles of all pairs, all heads.  All lanes of a warp.
+__device__ __forceinline__ int count_tiles(const KvWork& w) {
+  int sum = 0;
+  for (int pair = threadIdx.x & 31; pair < w.pairs; pair += 32) sum += tiles_of(w.extent_of(pair));
+  return __reduce_add_sync(0xffffffffu, sum) * w.heads;
 }
 // tiles per warp, at least `least`
-__device__ __forceinline__ int64_t share_of(int64_t total, int warps, int least) {
-  const int64_t s = (total + warps - 1) / warps;
-  return s < least ? least : s;
-}
+__device__ __forceinline__ int share_of(int total, int warps, int least) { return max(least, (total + warps - 1) / warps); }
 
-// A place in the sequence of tiles: a tile of an item, whose rows see `ext` keys.
+// A place in the sequence of tiles: a tile of an item, whose rows see `ext` keys of sequence b.
 struct KvCursor {
-  int pair, h, tile, ext;
-  __device__ __forceinline__ void next(const KvWork& w, int pairs) {
+  int pair, b, h, tile, ext;
+  __device__ __forceinline__ void next(const KvWork& w) {
     if (++tile * kTile < ext) return;
     tile = 0;
     if (++h < w.heads) return;
     h = 0;
     do {
       ++pair;
-      ext = pair < pairs ? w.extent_of(pair) : 1;
+      ext = pair < w.pairs ? w.extent_of(pair) : 1;
     } while (ext == 0);
+    b = w.by_row_tiles(pair);
   }
 };
-// ... the one that is `index` tiles from the first of all (there is one)
-__device__ __forceinline__ KvCursor find_tile(const KvWork& w, int pairs, int64_t index) {
-  KvCursor c;
-  int64_t before;
-  count_tiles(w, pairs, index, &c.pair, &before);
-  c.ext = w.extent_of(c.pair);
-  const int tiles = (c.ext + kTile - 1) / kTile;
-  c.h = static_cast<int>((index - before) / tiles);
-  c.tile = static_cast<int>(index - before - static_cast<int64_t>(c.h) * tiles);
+// ... the one that is `index` tiles from the first of all (there is one).  All lanes of a warp.
+__device__ __forceinline__ KvCursor find_tile(const KvWork& w, int index) {
+  const int lane = threadIdx.x & 31;
+  KvCursor c = {0, 0, 0, 0, 1};
+  int sum = 0;   // tiles of the pairs before these 32, for one head
+  for (int base = 0; base < w.pairs; base += 32) {
+    const int ext = base + lane < w.pairs ? w.extent_of(base + lane) : 0, n = tiles_of(ext);
+    int run = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    const uint32_t vote = __ballot_sync(0xffffffffu, (sum + run) * w.heads > index);
+    if (vote) {
+      const int src = __ffs(vote) - 1;   // the first whose tiles reach beyond `index`
+      const int in = index - __shfl_sync(0xffffffffu, sum + run - n, src) * w.heads, tiles = __shfl_sync(0xffffffffu, n, src);
+      c.pair = base + src;
+      c.b = w.by_row_tiles(c.pair);
+      c.ext = __shfl_sync(0xffffffffu, ext, src);
+      c.h = in / tiles;
+      c.tile = in - c.h * tiles;
+      break;
+    }
+    sum += __shfl_sync(0xffffffffu, run, 31);
+  }
   return c;
 }
 
-template <bool T16>
-__global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                     const __grid_constant__ CUtensorMap map_v, KvAttn p, KvWork work,
-                                                                     int pairs, float* parts) {
+// What a stream leaves for kv_combine_kernel: the item that its share ends in, if that item began in this stream and goes on in
+// the `more` streams behind it (pair -1: none).
+struct alignas(16) KvCut {
+  int pair, h, more, slot;
+};
+
+// What the producer warp tells the consumers of a stream about a tile.
+struct alignas(16) KvTileInfo {
+  int pair, h, tile, ext;
+  int there;                  // bit 0, 1: the first and second 16 keys are in the cache
+  int k_exp[2], v_exp[2];     // of the two halves
+  int b, unused[2];
+};
+
+// RW consumer warps share a stream of tiles (the rows of an item are theirs, 16 each); four consumer warps in all, and a
+// producer warp that looks up pages and exponents eight tiles ahead, a lane each, and keeps the rings filled.
+template <bool T16, int RW>
+__global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                  const __grid_constant__ CUtensorMap map_v,
+                                                                  const __grid_constant__ KvAttn p, const __grid_constant__ KvWork work,
+                                                                  float* parts, KvCut* cuts) {
+  constexpr int kStreams = kAttnWarps / RW, kStages = kAttnStages * RW;
   extern __shared__ uint8_t dyn[];
-  __shared__ uint64_t full[kAttnWarps][kAttnStages];
+  __shared__ uint64_t full[kStreams][kStages], empty[kStreams][kStages];
+  __shared__ KvTileInfo infos[kStreams][kInfoRing];
+  __shared__ int counts[kStreams], stream_share;
   __shared__ int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = dyn + ((1024u - (smem_u32(dyn) & 1023u)) & 1023u) + warp * (kAttnStages * kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* rings = dyn + ((1024u - (smem_u32(dyn) & 1023u)) & 1023u);
   if (threadIdx.x == 0) abort_flag = 0;
-  if (lane < kAttnStages) mbar_init(&full[warp][lane], 1);
-  if (lane == 0) fence_mbar_init();
-  __syncthreads();
+  if (threadIdx.x < kStreams * kStages) {
+    mbar_init(&full[0][0] + threadIdx.x, 1);
+    mbar_init(&empty[0][0] + threadIdx.x, RW);
+    fence_mbar_init();
+  }
   grid_wait();
-  const int n_warps = gridDim.x * kAttnWarps, me = blockIdx.x * kAttnWarps + warp;
+  const int n_streams = gridDim.x * kStreams, stream0 = blockIdx.x * kStreams;
+
+  if (warp == kAttnWarps) {
+    // ------------------------------------------------------------------ producer
+    constexpr int kLanes = 32 / kStreams, kAhead = 8;   // lanes of a stream; tiles of a round
+    const int st = lane / kLanes, j = lane % kLanes;
+    KvCursor c = {0, 0, 0, 0, 1};
+    int n_mine = 0;
+    if (parts) {
+      // equal shares of all tiles
+      const int total = count_tiles(work), share = share_of(total, n_streams, kMinShare);
+#pragma unroll 1
+      for (int x = 0; x < kStreams; ++x) {
+        const int64_t begin = static_cast<int64_t>(stream0 + x) * share;
+        if (begin >= total) break;
+        const KvCursor f = find_tile(work, static_cast<int>(begin));
+        if (st == x) c = f, n_mine = min(share, total - static_cast<int>(begin));
+      }
+      if (lane == 0) stream_share = share;
+    } else {
+      // short sequences: as many whole items for each stream
+      const int items = work.pairs * work.heads, per = (items + n_streams - 1) / n_streams;
+      const int item0 = min((stream0 + st) * per, items), item1 = min(item0 + per, items);
+      c.pair = work.by_heads(item0);
+      c.h = item0 - c.pair * work.heads;
+      for (int x = item0, pair = c.pair, h = c.h; x < item1; ++x) {
+        const int ext = work.extent_of(pair);
+        if (n_mine == 0) c.pair = pair, c.h = h, c.ext = ext;   // (the first item with keys)
+        n_mine += tiles_of(ext);
+        if (++h == work.heads) h = 0, ++pair;
+      }
+      c.b = work.by_row_tiles(c.pair);
+    }
+    if (j == 0) counts[st] = n_mine;
+    __syncthreads();
+    int most = n_mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    // lane j of a stream has its tiles j, j + 8, ...
+    for (int x = 0; x < j && x < kAhead; ++x)
+      if (x < n_mine) c.next(work);
+    uint8_t* ring = rings + st * (kStages * kStageBytes);
+    int stage = 0, phase = 0, next = 0;   // of the stream's next request (its first lane's)
+    bool gone = false;
+    for (int i0 = 0; i0 < most && !gone; i0 += kAhead) {
+      const int i = i0 + j;
+      if (j < kAhead && i < n_mine) {
+        KvTileInfo x;
+        const int32_t* row = p.tab.row(c.b);
+        const int key = c.tile * kTile;
+        int page = kv_page(row, p.tab.width, p.pool.n_pages, key >> work.shift);
+        int block[2];
+        block[0] = block[1] = page < 0 ? -1 : page * work.heads + c.h;
+        if (T16) {
+          page = kv_page(row, p.tab.width, p.pool.n_pages, (key >> 4) + 1);
+          block[1] = page < 0 ? -1 : page * work.heads + c.h;
+        }
+        if ((block[0] < 0 || (T16 && block[1] < 0 && key + 16 < c.ext)) && p.status) *p.status = DSB_ERR_ARG;
+        x.pair = c.pair, x.h = c.h, x.tile = c.tile, x.ext = c.ext, x.b = c.b;
+        x.there = (block[0] >= 0 ? 1 : 0) | (block[1] >= 0 ? 2 : 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x.k_exp[h] = x.v_exp[h] = 0;
+          if (h == 1 && !T16) x.k_exp[1] = x.k_exp[0], x.v_exp[1] = x.v_exp[0];
+          else if (block[h] >= 0) x.k_exp[h] = p.pool.k_exp[block[h]], x.v_exp[h] = p.pool.v_exp[block[h]];
+        }
+        x.unused[0] = block[0], x.unused[1] = block[1];
+        infos[st][i % kInfoRing] = x;
+        for (int y = 0; y < kAhead; ++y)
+          if (i + y + 1 < n_mine) c.next(work);
+      }
+      __syncwarp();
+      // the first lane of each stream requests the round's tiles as stages come free
+      const int upto = min(i0 + kAhead, n_mine);
+      const long long t0 = clock64();
+      while (__any_sync(0xffffffffu, j == 0 && next < upto)) {
+        bool moved = false;
+        if (j == 0 && next < upto && mbar_try_wait(&empty[st][stage], phase ^ 1)) {
+          const KvTileInfo& x = infos[st][next % kInfoRing];
+          uint64_t* bar = &full[st][stage];
+          uint8_t* k = ring + stage * kStageBytes;
+          uint8_t* v = k + kTile * kD;
+          const int b0 = x.unused[0], b1 = x.unused[1];
+          if (T16) {
+            const int bytes = ((b0 >= 0) + (b1 >= 0)) * 2 * 16 * kD;
+            if (bytes == 0) {
+              mbar_arrive(bar);
+            } else {
+              mbar_expect_tx(bar, bytes);
+              if (b0 >= 0) tma_load_2d(k, &map_k, bar, 0, b0 * 16), tma_load_2d(v, &map_v, bar, 0, b0 * 16);
+              if (b1 >= 0) tma_load_2d(k + 16 * kD, &map_k, bar, 0, b1 * 16), tma_load_2d(v + 16 * kD, &map_v, bar, 0, b1 * 16);
+            }
+          } else if (b0 < 0) {
+            mbar_arrive(bar);
+          } else {
+            const int y = (b0 << work.shift) + ((x.tile * kTile) & (work.T - 1));
+            mbar_expect_tx(bar, kStageBytes);
+            tma_load_2d(k, &map_k, bar, 0, y);
+            tma_load_2d(v, &map_v, bar, 0, y);
+          }
+          ++next;
+          if (++stage == kStages) stage = 0, phase ^= 1;
+          moved = true;
+        }
+        if (!__any_sync(0xffffffffu, moved)) {
+          const bool late = clock64() - t0 > kWaitLimitCycles * 2;
+          if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int*>(&abort_flag) != 0)) {
+            abort_flag = 1;
+            gone = true;
+            break;
+          }
+        }
+      }
+    }
+    if (gone && lane == 0 && p.status) *p.status = DSB_ERR_TIMEOUT;
+    // copies that are still on their way must not land in shared memory of whoever comes next
+    if (j == 0)
+      for (int back = min(next, kStages); back > 0; --back) {
+        const int x = next - back;
+        const long long t1 = clock64();
+        while (!mbar_try_wait_suspended(&full[st][x % kStages], (x / kStages) & 1) && clock64() - t1 < kWaitLimitCycles) {}
+      }
+    return;
+  }
+
+  // -------------------------------------------------------------------- consumers
+  const int g = lane >> 2, t = lane & 3, st = warp / RW, sub = warp % RW;
   // a length outside its table is reported once, by the first warp
-  if (me == 0 && p.lens && p.status)
+  if (blockIdx.x == 0 && warp == 0 && p.lens && p.status)
     for (int b = lane; b < p.B; b += 32)
       if (!kv_length_ok(p.lens[b], work.capacity)) *p.status = DSB_ERR_ARG;
   // rows that see no key
-  for (int pair = me; pair < pairs; pair += n_warps) {
+  for (int pair = blockIdx.x * kAttnWarps + warp; pair < work.pairs; pair += gridDim.x * kAttnWarps) {
     if (work.extent_of(pair) > 0) continue;
-    const int b = pair / work.row_tiles, row0 = (pair - b * work.row_tiles) * kRowTile;
-    for (int x = lane; x < kRowTile * work.heads * 16; x += 32) {
-      const int c = x & 15, h = (x >> 4) % work.heads, row = row0 + (x >> 4) / work.heads, qi = row / work.G;
+    const int b = work.by_row_tiles(pair), row0 = (pair - b * work.row_tiles) * work.rows_tile;
+#pragma unroll 1
+    for (int x = lane; x < work.rows_tile * work.heads * 16; x += 32) {
+      const int c = x & 15, r = work.by_heads(x >> 4), h = (x >> 4) - r * work.heads, row = row0 + r, qi = work.by_G(row);
       if (row < work.Sq * work.G)
         reinterpret_cast<uint4*>(p.o + b * p.o_sb + qi * p.o_ss + (h * work.G + row - qi * work.G) * p.o_sh)[c] = make_uint4(0, 0, 0, 0);
     }
   }
-  const int64_t total = count_tiles(work, pairs, 0, nullptr, nullptr);
-  const int64_t share = share_of(total, n_warps, parts ? kMinShare : 1);
-  int64_t first = me * share, end = min(first + share, total);
-  if (first >= total) return;
-  KvCursor fetch = find_tile(work, pairs, first);
-  if (!parts) {
-    // nothing is cut: the items that begin in this share, to their ends
-    if (fetch.tile > 0) {
-      first += (fetch.ext + kTile - 1) / kTile - fetch.tile;
-      if (first >= end) return;
-      fetch = find_tile(work, pairs, first);
-    }
-    if (end < total) {
-      const KvCursor last = find_tile(work, pairs, end);
-      if (last.tile > 0) end += (last.ext + kTile - 1) / kTile - last.tile;
-    }
-  }
-  const int n_mine = static_cast<int>(end - first);
-  KvCursor at = fetch;
-
-  // block (page * heads + head) of the 16 keys from `key` on, or -1
-  auto block_of = [&](const KvCursor& c, int key) {
-    const int page = kv_page(p.tab.row(c.pair / work.row_tiles), p.tab.width, p.pool.n_pages, key / work.T);
-    return page < 0 ? -1 : page * work.heads + c.h;
-  };
-  struct Tile {
-    int block0, block1;   // of the first and second 16 keys
-  };
-  auto look_up = [&](const KvCursor& c) {
-    Tile x;
-    x.block0 = block_of(c, c.tile * kTile);
-    x.block1 = x.block0;
-    if (T16) x.block1 = c.tile * kTile + 16 < work.capacity ? block_of(c, c.tile * kTile + 16) : -1;
-    return x;
-  };
-  auto issue = [&](const Tile& x, const KvCursor& c, int stage) {
-    if (lane == 0) {
-      const int tile = c.tile;
-      if ((x.block0 < 0 || (T16 && x.block1 < 0 && tile * kTile + 16 < c.ext)) && p.status) *p.status = DSB_ERR_ARG;
-      uint64_t* bar = &full[warp][stage];
-      uint8_t* k = ring + stage * kStageBytes;
-      uint8_t* v = k + kTile * kD;
-      const int slot = (tile * kTile) & (work.T - 1);
-      if (T16) {
-        const int bytes = ((x.block0 >= 0) + (x.block1 >= 0)) * 2 * 16 * kD;
-        if (bytes == 0) {
-          mbar_arrive(bar);
-        } else {
-          mbar_expect_tx(bar, bytes);
-          if (x.block0 >= 0) tma_load_2d(k, &map_k, bar, 0, x.block0 * 16), tma_load_2d(v, &map_v, bar, 0, x.block0 * 16);
-          if (x.block1 >= 0)
-            tma_load_2d(k + 16 * kD, &map_k, bar, 0, x.block1 * 16), tma_load_2d(v + 16 * kD, &map_v, bar, 0, x.block1 * 16);
-        }
-      } else if (x.block0 < 0) {
-        mbar_arrive(bar);
-      } else {
-        mbar_expect_tx(bar, kStageBytes);
-        tma_load_2d(k, &map_k, bar, 0, x.block0 * work.T + slot);
-        tma_load_2d(v, &map_v, bar, 0, x.block0 * work.T + slot);
-      }
-    }
-  };
-
-  // tiles on their way: [0] is the one to be multiplied next
-  Tile line[kAttnStages];
-  int issued = 0;
-#pragma unroll
-  for (int s = 0; s < kAttnStages; ++s) {
-    line[s].block0 = line[s].block1 = -1;
-    if (s < n_mine) {
-      line[s] = look_up(fetch);
-      issue(line[s], fetch, s);
-      ++issued;
-      fetch.next(work, pairs);
-    }
-  }
-  Tile ahead = {-1, -1};
-  if (issued < n_mine) ahead = look_up(fetch);
-  struct Exps {
-    int k0, k1, v0, v1;
-  };
-  auto exps_of = [&](const Tile& x) {
-    Exps e = {0, 0, 0, 0};
-    if (x.block0 >= 0) e.k0 = p.pool.k_exp[x.block0], e.v0 = p.pool.v_exp[x.block0];
-    if (T16) {
-      if (x.block1 >= 0) e.k1 = p.pool.k_exp[x.block1], e.v1 = p.pool.v_exp[x.block1];
-    } else {
-      e.k1 = e.k0, e.v1 = e.v0;
-    }
-    return e;
-  };
-  Exps exps = exps_of(line[0]);
+  __syncthreads();
+  const int n_mine = counts[st];
+  const uint8_t* ring = rings + st * (kStages * kStageBytes);
 
   uint32_t q[8][4];          // A fragments of 8 x 16 columns: lane (g, t) has rows g, g + 8 and columns 32 t + 4 i + 0..3 of them
   float c_row[2];            // sm_scale * log2(e) * the power of two that the row was divided by
-  int seen[2], all_see = 0;  // keys that the rows g, g + 8 see; that every row of the tile sees
+  int seen[2], all_see = 0, any_see = 0;  // keys that the rows g, g + 8 see; that every row of the warp sees; that its last one does
   float o[16][4], m_ref[2], l_sum[2];
-
-  int stage = 0, parity = 0, seg_first = at.tile;
-  bool failed = false, fresh = true;
+  int stage = 0, parity = 0, seg_first = 0;
+  bool fresh = true;
   for (int i = 0; i < n_mine; ++i) {
+    if (!mbar_wait_all(&full[st][stage], parity, &abort_flag)) {
+      if (lane == 0 && p.status) *p.status = DSB_ERR_TIMEOUT;
+      return;
+    }
+    const int4 info0 = *reinterpret_cast<const int4*>(&infos[st][i % kInfoRing]);      // pair, h, tile, ext
+    const int4 info1 = *(reinterpret_cast<const int4*>(&infos[st][i % kInfoRing]) + 1);  // there, k_exp, v_exp[0]
+    const int2 info2 = *reinterpret_cast<const int2*>(reinterpret_cast<const int*>(&infos[st][i % kInfoRing]) + 8);   // v_exp[1], b
+    const int b = info2.y, rt = info0.x - b * work.row_tiles, head = info0.y, ext = info0.w, key0 = info0.z * kTile;
+    const int row0 = rt * work.rows_tile + sub * kRowTile;
     if (fresh) {
       // ---- an item begins: its rows
-      const int b = at.pair / work.row_tiles, rt = at.pair - b * work.row_tiles, rows = work.Sq * work.G;
-      const int len = work.length(b);
-      all_see = kv_visible(len, work.Sq, rt * kRowTile / work.G, work.causal);
+      seg_first = info0.z;
+      const int len = work.length(b), rows = work.Sq * work.G;
+      all_see = kv_visible(len, work.Sq, work.by_G(min(row0, rows - 1)), work.causal);
+      any_see = row0 < rows ? kv_visible(len, work.Sq, work.by_G(min(row0 + kRowTile, rows) - 1), work.causal) : 0;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int row = rt * kRowTile + g + 8 * r, qi = row / work.G;
+        const int row = row0 + g + 8 * r, qi = work.by_G(row);
         uint4 raw[4];
         raw[0] = raw[1] = raw[2] = raw[3] = make_uint4(0, 0, 0, 0);
         seen[r] = 0;
         if (row < rows) {
           seen[r] = kv_visible(len, work.Sq, qi, work.causal);
-          const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_sb + qi * p.q_ss + (at.h * work.G + row - qi * work.G) * p.q_sh + 32 * t);
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_sb + qi * p.q_ss + (head * work.G + row - qi * work.G) * p.q_sh + 32 * t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) raw[j] = src[j];
         }
-        float top = 0.f;
+        uint32_t most = 0;   // magnitudes as bits, two at a time (NaN is more than any: its row is NaN whatever it is divided by)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(u[e]);
-            if (fabsf(f.x) < INFINITY) top = fmaxf(top, fabsf(f.x));
-            if (fabsf(f.y) < INFINITY) top = fmaxf(top, fabsf(f.y));
-          }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        for (int j = 0; j < 4; ++j)
+          most = __vmaxu2(__vmaxu2(most, __vmaxu2(raw[j].x & 0x7fff7fffu, raw[j].y & 0x7fff7fffu)),
+                          __vmaxu2(raw[j].z & 0x7fff7fffu, raw[j].w & 0x7fff7fffu));
+        most = max(most >> 16, most & 0xffffu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
         // the row over 2^eq has its largest magnitude in [2^13, 2^14); eq is kept where both 2^eq and 2^-eq are ordinary numbers
-        int eq = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 13;
+        int eq = static_cast<int>(most >> 7) - 127 - 13;
         eq = max(-100, min(114, eq));
         const float down = pow2i(-eq);
         c_row[r] = p.scale_log2 * pow2i(eq);
@@ -502,28 +576,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
       for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
       fresh = false;
     }
-    // exponents of the tile after this one, and the place of the one that will be requested after it
-    const Exps exps_next = exps_of(line[1]);
-
-    if (!mbar_wait_all(&full[warp][stage], parity, &abort_flag)) {
-      failed = true;
-      break;
-    }
     const uint8_t* ks = ring + stage * kStageBytes;
     const uint8_t* vs = ks + kTile * kD;
-    const int key0 = at.tile * kTile;
-    const bool whole = key0 + kTile <= all_see && line[0].block0 >= 0 && line[0].block1 >= 0;
-
+    const bool whole = key0 + kTile <= all_see && info1.x == 3;
+    if (key0 < any_see) {
     // ---- scores: n tile j holds keys 8 j + g as columns
     float s[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      const uint8_t* row = ks + (8 * j + g) * kD;
+    for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         // chunk 2 t + c of the key's row lies at 2 t + c xor g (the swizzle): no two lanes of an eight share banks
-        const uint4 w = *reinterpret_cast<const uint4*>(row + (((2 * t + c) ^ g) << 4));
+        const uint4 w = *reinterpret_cast<const uint4*>(ks + (8 * j + g) * kD + (((2 * t + c) ^ g) << 4));
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -534,40 +600,35 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
       }
     }
     // ---- t = S c + ev, masked; the running reference
-    float inv_v[2];   // 2^-ev of the two halves
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int ek = hf ? exps.k1 : exps.k0, ev = hf ? exps.v1 : exps.v0;
-      inv_v[hf] = pow2i(-ev);
-      const float f0 = c_row[0] * pow2i(ek), f1 = c_row[1] * pow2i(ek), add = static_cast<float>(ev);
+      const float kf = pow2i(hf ? info1.z : info1.y), add = static_cast<float>(hf ? info2.x : info1.w);
+      const float f0 = c_row[0] * kf, f1 = c_row[1] * kf;
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         const int j = 2 * hf + jj;
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], e < 2 ? f0 : f1, add);
         if (!whole) {
-          const bool there = hf ? line[0].block1 >= 0 : line[0].block0 >= 0;
+          const bool there = info1.x & (1 << hf);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (!there || key0 + 8 * j + 2 * t + (e & 1) >= seen[e >> 1]) s[j][e] = -INFINITY;
         }
-        top[0] = fmaxf(top[0], fmaxf(s[j][0], s[j][1]));
-        top[1] = fmaxf(top[1], fmaxf(s[j][2], s[j][3]));
+        top[0] = max3f(top[0], s[j][0], s[j][1]);
+        top[1] = max3f(top[1], s[j][2], s[j][3]);
       }
     }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m_ref[0] || top[1] > m_ref[1])) {
+    if (__any_sync(0xffffffffu, top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack)) {
       float f[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float m_new = fmaxf(m_ref[r], top[r]);
-        f[r] = m_new == m_ref[r] ? 1.f : fast_exp2(m_ref[r] - m_new);   // (0 for the first keys of a row)
-        m_ref[r] = m_new;
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        const bool moves = top[r] > m_ref[r] + kSlack;
+        f[r] = moves ? fast_exp2(m_ref[r] - top[r]) : 1.f;   // (0 for the first keys of a row)
+        m_ref[r] = moves ? top[r] : m_ref[r];
         l_sum[r] *= f[r];
       }
 #pragma unroll
@@ -578,6 +639,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
     uint32_t a[2][4];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
+      const float inv_v = pow2i(-(hf ? info2.x : info1.w));
       float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
@@ -589,8 +651,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
         a[hf][2 * jj] = pack_f16x2(s[j][0], s[j][1]);
         a[hf][2 * jj + 1] = pack_f16x2(s[j][2], s[j][3]);
       }
-      l_sum[0] = fmaf(sum0, inv_v[hf], l_sum[0]);
-      l_sum[1] = fmaf(sum1, inv_v[hf], l_sum[1]);
+      l_sum[0] = fmaf(sum0, inv_v, l_sum[0]);
+      l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
     }
     // ---- O += P V: n tile n holds columns 16 g + n
 #pragma unroll
@@ -601,7 +663,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
         const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
         w[x] = *reinterpret_cast<const uint4*>(vs + key * kD + ((g ^ (key & 7)) << 4));
         // behind the last key there may be anything, and 0 * NaN is NaN
-        if (!whole && (key0 + key >= at.ext || (hf ? line[0].block1 : line[0].block0) < 0)) w[x] = make_uint4(0, 0, 0, 0);
+        if (!whole && (key0 + key >= ext || !(info1.x & (1 << hf)))) w[x] = make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -618,39 +680,28 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
         for (int e = 0; e < 4; ++e) mma_16816(o[4 * c + e], a[hf], b0[e], b1[e]);
       }
     }
-    __syncwarp();
-    // ---- this stage is free: the next request, and the look-up of the one behind it
-#pragma unroll
-    for (int x = 0; x + 1 < kAttnStages; ++x) line[x] = line[x + 1];
-    line[kAttnStages - 1] = ahead;
-    if (issued < n_mine) {
-      issue(ahead, fetch, stage);
-      ++issued;
-      fetch.next(work, pairs);
-      if (issued < n_mine) ahead = look_up(fetch);
     }
-    exps = exps_next;
-    if (++stage == kAttnStages) stage = 0, parity ^= 1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[st][stage]);
+    if (++stage == kStages) stage = 0, parity ^= 1;
 
-    // ---- the end of an item, or of this warp's share of it
-    const KvCursor here = at;
-    at.next(work, pairs);
-    if (at.tile == 0 || i + 1 == n_mine) {
+    // ---- the end of an item, or of this stream's share of it
+    const bool last = key0 + kTile >= ext;
+    if (last || i + 1 == n_mine) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 1);
         l_sum[r] += __shfl_xor_sync(0xffffffffu, l_sum[r], 2);
       }
-      const int b = here.pair / work.row_tiles, rt = here.pair - b * work.row_tiles;
-      const bool alone = seg_first == 0 && (here.tile + 1) * kTile >= here.ext;
+      const bool alone = seg_first == 0 && last;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int row = rt * kRowTile + g + 8 * r, qi = row / work.G;
+        const int row = row0 + g + 8 * r, qi = work.by_G(row);
         if (row >= work.Sq * work.G) continue;
         // columns 32 t + n of the row are o[n][2 r], columns 32 t + 16 + n are o[n][2 r + 1]
         if (alone) {
           const float inv = m_ref[r] == -INFINITY ? 0.f : 1.f / l_sum[r];
-          uint4* dst = reinterpret_cast<uint4*>(p.o + b * p.o_sb + qi * p.o_ss + (here.h * work.G + row - qi * work.G) * p.o_sh + 32 * t);
+          uint4* dst = reinterpret_cast<uint4*>(p.o + b * p.o_sb + qi * p.o_ss + (head * work.G + row - qi * work.G) * p.o_sh + 32 * t);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -661,9 +712,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
               dst[2 * c + e] = make_uint4(u[0], u[1], u[2], u[3]);
             }
         } else {
-          // slot 0: the part with which this warp's share begins, 1: the one with which it ends
-          const int slot = first + i + 1 - (here.tile + 1 - seg_first) == first ? 0 : 1;
-          float* dst = parts + ((static_cast<int64_t>(me) * 2 + slot) * kRowTile + g + 8 * r) * kPartRow;
+          // slot 0: the part with which this stream's share begins, 1: the one with which it ends
+          const int slot = i == info0.z - seg_first ? 0 : 1;
+          float* dst = parts + ((static_cast<int64_t>((stream0 + st) * RW + sub) * 2 + slot) * kRowTile + g + 8 * r) * kPartRow;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -673,69 +724,68 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 2) kv_attn_kernel(const __gri
           if (t == 0) dst[128] = m_ref[r], dst[129] = l_sum[r];
         }
       }
-      seg_first = 0;
+      if (parts && i + 1 == n_mine && sub == 0 && lane == 0) {
+        const int border = info0.z + 1, rest = tiles_of(ext) - border;
+        cuts[stream0 + st] = {!last && seg_first == 0 ? info0.x : -1, head, (rest + stream_share - 1) / stream_share, i == info0.z ? 0 : 1};
+      }
       fresh = true;
     }
   }
-  if (failed) {
-    if (lane == 0 && p.status) *p.status = DSB_ERR_TIMEOUT;
-    // copies that are still on their way must not land in shared memory of whoever comes next
-    for (int s = 0; s < kAttnStages; ++s) {
-      const int st = stage + s < kAttnStages ? stage + s : stage + s - kAttnStages;
-      const int64_t t0 = clock64();
-      while (!mbar_try_wait(&full[warp][st], st >= stage ? parity : parity ^ 1) && clock64() - t0 < kWaitLimitCycles) {}
-    }
-  }
+  if (parts && n_mine == 0 && sub == 0 && lane == 0) cuts[stream0 + st] = {-1, 0, 0, 0};
 }
 
-// Items that several warps shared: CTA w has the one that the border between the shares of warps w and w + 1 cuts, if that is
-// its first cut.  One warp per row; the parts, in order, brought to one reference.
-__global__ void __launch_bounds__(256) kv_combine_kernel(KvAttn p, KvWork work, int pairs, int n_warps, const float* parts) {
+// Items that several streams shared: CTA (w, y) has rows y, y + gridDim.y, ... of the item that stream w was the first to leave
+// unfinished.  Its warps take the parts (a stream's each) in turn, brought to one reference; the warps' sums are added in order.
+__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ KvAttn p, const __grid_constant__ KvWork work,
+                                                         const float* parts, const KvCut* cuts) {
   grid_wait();
-  __shared__ KvCursor item;
-  __shared__ int64_t item_share;
-  if (threadIdx.x < 32) {
-    const int64_t total = count_tiles(work, pairs, 0, nullptr, nullptr), share = share_of(total, n_warps, kMinShare);
-    const int64_t border = (blockIdx.x + 1) * share;
-    KvCursor c = {-1, 0, 0, 0};
-    if (border < total) {
-      c = find_tile(work, pairs, border);
-      if (c.tile == 0 || c.tile > share) c.pair = -1;
-    }
-    if (threadIdx.x == 0) item = c, item_share = share;
-  }
-  __syncthreads();
-  if (item.pair < 0) return;
-  const int lane = threadIdx.x & 31, h = item.h, b = item.pair / work.row_tiles, rt = item.pair - b * work.row_tiles;
-  // the item's first tile lies item.tile tiles before the border, in the share of warp blockIdx.x (which starts with it if the
-  // whole share is before the border)
-  const int64_t w0 = blockIdx.x, tiles = (item.ext + kTile - 1) / kTile;
-  const int64_t w1 = ((w0 + 1) * item_share - item.tile + tiles - 1) / item_share;
-  const int slot0 = item.tile == item_share ? 0 : 1;
-  for (int r = threadIdx.x >> 5; r < kRowTile; r += 8) {
-    const int row = rt * kRowTile + r, qi = row / work.G;
-    if (row >= work.Sq * work.G) return;
-    auto part = [&](int64_t w) { return parts + ((w * 2 + (w == w0 ? slot0 : 0)) * kRowTile + r) * kPartRow; };
+  const KvCut cut = cuts[blockIdx.x];
+  if (cut.pair < 0) return;
+  __shared__ float4 sums[8][32];
+  __shared__ float tops[8], lens[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = work.by_row_tiles(cut.pair), row0 = (cut.pair - b * work.row_tiles) * work.rows_tile;
+  const int rw = work.rows_tile / kRowTile, rows = min(work.rows_tile, work.Sq * work.G - row0), w0 = blockIdx.x, n = cut.more + 1;
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    auto part = [&](int i) {
+      return parts + (((static_cast<int64_t>(w0 + i) * rw + r / kRowTile) * 2 + (i == 0 ? cut.slot : 0)) * kRowTile + r % kRowTile) * kPartRow;
+    };
     float m = -INFINITY;
-    for (int64_t w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, part(w)[128]);
+    for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, part(i)[128]);
     m = warp_max(m);
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, tops[i]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
     if (m != -INFINITY) {
 #pragma unroll 4
-      for (int64_t w = w0; w <= w1; ++w) {
-        const float* src = part(w);
+      for (int i = warp; i < n; i += 8) {
+        const float* src = part(i);
         const float f = fast_exp2(src[128] - m);
         const float4 v = reinterpret_cast<const float4*>(src)[lane];
         o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
         l = fmaf(src[129], f, l);
       }
     }
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    uint2 u;
-    u.x = pack_bf16x2(o.x * inv, o.y * inv);
-    u.y = pack_bf16x2(o.z * inv, o.w * inv);
-    reinterpret_cast<uint2*>(p.o + b * p.o_sb + qi * p.o_ss + (h * work.G + row - qi * work.G) * p.o_sh)[lane] = u;
+    sums[warp][lane] = o;
+    if (lane == 0) lens[warp] = l;
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        const float4 v = sums[i][lane];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        l += lens[i];
+      }
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      uint2 u;
+      u.x = pack_bf16x2(o.x * inv, o.y * inv);
+      u.y = pack_bf16x2(o.z * inv, o.w * inv);
+      const int row = row0 + r, qi = work.by_G(row);
+      reinterpret_cast<uint2*>(p.o + b * p.o_sb + qi * p.o_ss + (cut.h * work.G + row - qi * work.G) * p.o_sh)[lane] = u;
+    }
+    __syncthreads();
   }
 }
 
@@ -848,9 +898,12 @@ static int attn_warps() {
   int n = cached[dev].load();
   if (n > 0) return n;
   int per_sm = 0;
-  if (cudaFuncSetAttribute(kv_attn_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnDynSmem) != cudaSuccess ||
-      cudaFuncSetAttribute(kv_attn_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnDynSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_attn_kernel<false>, kAttnWarps * 32, kAttnDynSmem) != cudaSuccess ||
+  auto opt_in = [](auto kern) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnDynSmem) == cudaSuccess;
+  };
+  if (!opt_in(kv_attn_kernel<false, 1>) || !opt_in(kv_attn_kernel<false, 2>) || !opt_in(kv_attn_kernel<false, 4>) ||
+      !opt_in(kv_attn_kernel<true, 1>) || !opt_in(kv_attn_kernel<true, 2>) || !opt_in(kv_attn_kernel<true, 4>) ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_attn_kernel<false, 1>, kAttnThreads, kAttnDynSmem) != cudaSuccess ||
       per_sm <= 0)
     return 0;
   n = sm_count() * per_sm * kAttnWarps;
@@ -859,7 +912,7 @@ static int attn_warps() {
 }
 
 extern "C" int64_t dsb_kv_attn_workspace_bytes(void) {
-  return static_cast<int64_t>(attn_warps()) * 2 * kRowTile * kPartRow * 4;
+  return static_cast<int64_t>(attn_warps()) * (2 * kRowTile * kPartRow * 4 + sizeof(KvCut));
 }
 
 extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_stride_b, int64_t q_stride_s, int64_t q_stride_h,
@@ -888,15 +941,25 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   p.causal = causal ? 1 : 0;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.status = status;
-  const int64_t rows = static_cast<int64_t>(Sq) * p.G, row_tiles = (rows - 1) / kRowTile + 1, pairs = row_tiles * B;
-  if (rows > 0x7fffff00 || pairs > 0x7fffffff) return DSB_ERR_UNSUPPORTED;
+  const int64_t rows = static_cast<int64_t>(Sq) * p.G;
+  if (rows > 1 << 30) return DSB_ERR_UNSUPPORTED;
+  // 16 rows of an item for each of up to four warps that share its keys
+  const int rw = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t row_tiles = (rows - 1) / (kRowTile * rw) + 1, pairs = row_tiles * B;
+  if (pairs > 0x3fffffff || pairs * row_tiles >= 1ll << 45) return DSB_ERR_UNSUPPORTED;
   KvWork w = {};
   w.Sq = Sq;
   w.G = p.G;
   w.heads = p.pool.heads;
   w.T = p.pool.T;
+  w.shift = w.T == 16 ? 4 : w.T == 32 ? 5 : w.T == 64 ? 6 : 7;
+  w.pairs = static_cast<int>(pairs);
   w.causal = p.causal;
+  w.rows_tile = kRowTile * rw;
   w.row_tiles = static_cast<int>(row_tiles);
+  w.by_G = FastDiv::of(p.G);
+  w.by_row_tiles = FastDiv::of(w.row_tiles);
+  w.by_heads = FastDiv::of(w.heads);
   w.capacity = p.tab.capacity(p.pool.T);
   w.lens = lens;
   w.len_all = len_all;
@@ -905,11 +968,14 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   const int64_t most_len = lens ? w.capacity : len_all, item_tiles = (most_len + kTile - 1) / kTile;
   const int64_t items = pairs * p.pool.heads;
   const bool cut = item_tiles > kMinShare;
+  if (items > 0x3fffffff || items * item_tiles > 0x3fffffff) return DSB_ERR_UNSUPPORTED;
   if (cut && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))) return DSB_ERR_ARG;
   const int warps = attn_warps();
   if (warps <= 0) return DSB_ERR_CUDA;
   if (cut && workspace_bytes < dsb_kv_attn_workspace_bytes()) return DSB_ERR_ARG;
-  int64_t ctas = cut ? (items * item_tiles + kMinShare * kAttnWarps - 1) / (kMinShare * kAttnWarps) : (items + kAttnWarps - 1) / kAttnWarps;
+  const int streams_cta = kAttnWarps / rw;
+  const int64_t streams = cut ? (items * item_tiles + kMinShare - 1) / kMinShare : items;
+  int64_t ctas = (streams + streams_cta - 1) / streams_cta;
   if (ctas < 1) ctas = 1;
   if (ctas > warps / kAttnWarps) ctas = warps / kAttnWarps;
   const uint64_t map_rows = static_cast<uint64_t>(p.pool.n_pages) * p.pool.heads * p.pool.T;
@@ -918,13 +984,17 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   if ((rc = make_tmap_2d(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.pool.k, map_rows, kD, kD, box, kD)) != DSB_OK) return rc;
   if ((rc = make_tmap_2d(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.pool.v, map_rows, kD, kD, box, kD)) != DSB_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int n_pairs = static_cast<int>(pairs);
   float* parts = cut ? reinterpret_cast<float*>(workspace) : nullptr;
-  cudaError_t err = launch_kernel(p.pool.T == 16 ? kv_attn_kernel<true> : kv_attn_kernel<false>, static_cast<unsigned>(ctas),
-                                  kAttnWarps * 32, kAttnDynSmem, st, mk, mv, p, w, n_pairs, parts);
+  auto kern = p.pool.T == 16 ? (rw == 1 ? kv_attn_kernel<true, 1> : rw == 2 ? kv_attn_kernel<true, 2> : kv_attn_kernel<true, 4>)
+                             : (rw == 1 ? kv_attn_kernel<false, 1> : rw == 2 ? kv_attn_kernel<false, 2> : kv_attn_kernel<false, 4>);
+  const int n_streams = static_cast<int>(ctas) * streams_cta;
+  KvCut* cuts = reinterpret_cast<KvCut*>(parts + static_cast<int64_t>(warps) * 2 * kRowTile * kPartRow);
+  cudaError_t err = launch_kernel(kern, static_cast<unsigned>(ctas), kAttnThreads, kAttnDynSmem, st, mk, mv, p, w, parts, cuts);
   if (err != cudaSuccess) return DSB_ERR_CUDA;
-  const int n_warps = static_cast<int>(ctas) * kAttnWarps;
-  if (cut && n_warps > 1)
-    err = launch_kernel(kv_combine_kernel, n_warps - 1, 256, 0, st, p, w, n_pairs, n_warps, static_cast<const float*>(parts));
+  if (cut && n_streams > 1) {
+    const int rows_cta = static_cast<int>(rows < 16 ? rows : 16);
+    err = launch_kernel(kv_combine_kernel, dim3(n_streams - 1, rows_cta), 256, 0, st, p, w, static_cast<const float*>(parts),
+                        static_cast<const KvCut*>(cuts));
+  }
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }

@@ -138,7 +138,8 @@ ATT = [
     (1, 1, 1, 1, 16, [1], False), (1, 1, 2, 2, 16, [77], False), (2, 1, 8, 2, 64, [0, 65], False), (3, 1, 5, 1, 32, [31, 32, 33], True),
     (2, 3, 8, 8, 128, [127, 2], True), (1, 5, 10, 2, 64, [300], True), (2, 16, 4, 4, 16, [16, 250], False), (2, 17, 16, 2, 64, [17, 500], True),
     (1, 70, 4, 2, 32, [64], True), (2, 130, 3, 3, 64, [129, 400], False), (1, 1, 64, 4, 64, [2100], False), (5, 2, 24, 3, 128, [1, 1300, 0, 257, 640], True),
-    (1, 1, 2, 1, 64, [9000], False), (1, 300, 2, 1, 64, [40], True),
+    (1, 1, 2, 1, 64, [9000], False), (1, 300, 2, 1, 64, [40], True), (1, 20, 4, 2, 16, [45], True), (2, 3, 8, 1, 16, [700, 5], True),
+    (1, 3, 10, 1, 64, [3000], False), (2, 33, 2, 1, 128, [2500, 1200], True), (70, 1, 3, 3, 16, [9 * i % 40 for i in range(70)], False),
 ]
 
 

@@ -401,16 +401,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
       c.b = work.by_row_tiles(c.pair);
     }
     if (j == 0) counts[st] = n_mine;
-    __syncthreads();
     int most = n_mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     // lane j of a stream has its tiles j, j + 8, ...
+#pragma unroll 1
     for (int x = 0; x < j && x < kAhead; ++x)
       if (x < n_mine) c.next(work);
     uint8_t* ring = rings + st * (kStages * kStageBytes);
     int stage = 0, phase = 0, next = 0;   // of the stream's next request (its first lane's)
     bool gone = false;
+    if (most == 0) __syncthreads();
     for (int i0 = 0; i0 < most && !gone; i0 += kAhead) {
       const int i = i0 + j;
       if (j < kAhead && i < n_mine) {
@@ -435,9 +436,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
         }
         x.unused[0] = block[0], x.unused[1] = block[1];
         infos[st][i % kInfoRing] = x;
+#pragma unroll 1
         for (int y = 0; y < kAhead; ++y)
           if (i + y + 1 < n_mine) c.next(work);
       }
+      if (i0 == 0) __syncthreads();
       __syncwarp();
       // the first lane of each stream requests the round's tiles as stages come free
       const int upto = min(i0 + kAhead, n_mine);
@@ -519,11 +522,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
   float o[16][4], m_ref[2], l_sum[2];
   int stage = 0, parity = 0, seg_first = 0;
   bool fresh = true;
+  auto arrived = [&] {
+    if (mbar_wait_all(&full[st][stage], parity, &abort_flag)) return true;
+    if (lane == 0 && p.status) *p.status = DSB_ERR_TIMEOUT;
+    return false;
+  };
   for (int i = 0; i < n_mine; ++i) {
-    if (!mbar_wait_all(&full[st][stage], parity, &abort_flag)) {
-      if (lane == 0 && p.status) *p.status = DSB_ERR_TIMEOUT;
-      return;
-    }
+    // (the first round's descriptions were written before the CTA's barrier: the first item's rows are fetched under its keys)
+    if (i > 0 && !arrived()) return;
     const int4 info0 = *reinterpret_cast<const int4*>(&infos[st][i % kInfoRing]);      // pair, h, tile, ext
     const int4 info1 = *(reinterpret_cast<const int4*>(&infos[st][i % kInfoRing]) + 1);  // there, k_exp, v_exp[0]
     const int2 info2 = *reinterpret_cast<const int2*>(reinterpret_cast<const int*>(&infos[st][i % kInfoRing]) + 8);   // v_exp[1], b
@@ -576,6 +582,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
       for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
       fresh = false;
     }
+    if (i == 0 && !arrived()) return;
     const uint8_t* ks = ring + stage * kStageBytes;
     const uint8_t* vs = ks + kTile * kD;
     const bool whole = key0 + kTile <= all_see && info1.x == 3;

@@ -278,12 +278,13 @@ struct KvWork {
   }
 };
 __device__ __forceinline__ int tiles_of(int ext) { return (ext + kTile - 1) / kTile; }
-// Tiles of all pairs, all heads.  All lanes of a warp.
-__device__ __forceinline__ int count_tiles(const KvWork& w) {
+// Tiles of the first n pairs, all heads.  All lanes of a warp.
+__device__ __forceinline__ int count_tiles(const KvWork& w, int n) {
   int sum = 0;
-  for (int pair = threadIdx.x & 31; pair < w.pairs; pair += 32) sum += tiles_of(w.extent_of(pair));
+  for (int pair = threadIdx.x & 31; pair < n; pair += 32) sum += tiles_of(w.extent_of(pair));
   return __reduce_add_sync(0xffffffffu, sum) * w.heads;
 }
+__device__ __forceinline__ int count_tiles(const KvWork& w) { return count_tiles(w, w.pairs); }
 // tiles per warp, at least `least`
 __device__ __forceinline__ int share_of(int total, int warps, int least) { return max(least, (total + warps - 1) / warps); }
 
@@ -741,59 +742,79 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
   if (parts && n_mine == 0 && sub == 0 && lane == 0) cuts[stream0 + st] = {-1, 0, 0, 0};
 }
 
-// Items that several streams shared: CTA (w, y) has rows y, y + gridDim.y, ... of the item that stream w was the first to leave
-// unfinished.  Its warps take the parts (a stream's each) in turn, brought to one reference; the warps' sums are added in order.
-__global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ KvAttn p, const __grid_constant__ KvWork work,
-                                                         const float* parts, const KvCut* cuts) {
+// Items that several streams shared are brought together from their parts (a stream's each), in order.  Where an item has a few
+// parts, CTA (w, y) has eight rows, a warp each, of the item that stream w was the first to leave unfinished.  Where few items
+// have many parts, CTA (x, y) has row y of item x, and WARPS warps for it; it finds the item's streams itself.
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) kv_combine_kernel(const __grid_constant__ KvAttn p,
+                                                                                  const __grid_constant__ KvWork work, const float* parts,
+                                                                                  const KvCut* cuts, int n_streams) {
   grid_wait();
-  const KvCut cut = cuts[blockIdx.x];
-  if (cut.pair < 0) return;
-  __shared__ float4 sums[8][32];
-  __shared__ float tops[8], lens[8];
+  KvCut cut;
+  int w0 = blockIdx.x;
+  if constexpr (WARPS == 1) {
+    cut = cuts[w0];
+    if (cut.pair < 0) return;
+  } else {
+    cut.pair = work.by_heads(blockIdx.x);
+    cut.h = blockIdx.x - cut.pair * work.heads;
+    const int share = share_of(count_tiles(work), n_streams, kMinShare), tiles = tiles_of(work.extent_of(cut.pair));
+    const int first = count_tiles(work, cut.pair) + cut.h * tiles;
+    w0 = first / share;
+    cut.more = (first + tiles - 1) / share - w0;
+    cut.slot = first == w0 * share ? 0 : 1;
+    if (tiles == 0 || cut.more == 0) return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = work.by_row_tiles(cut.pair), row0 = (cut.pair - b * work.row_tiles) * work.rows_tile;
-  const int rw = work.rows_tile / kRowTile, rows = min(work.rows_tile, work.Sq * work.G - row0), w0 = blockIdx.x, n = cut.more + 1;
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    auto part = [&](int i) {
-      return parts + (((static_cast<int64_t>(w0 + i) * rw + r / kRowTile) * 2 + (i == 0 ? cut.slot : 0)) * kRowTile + r % kRowTile) * kPartRow;
-    };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 256) m = fmaxf(m, part(i)[128]);
-    m = warp_max(m);
-    if (lane == 0) tops[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, tops[i]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    if (m != -INFINITY) {
-#pragma unroll 4
-      for (int i = warp; i < n; i += 8) {
-        const float* src = part(i);
-        const float f = fast_exp2(src[128] - m);
-        const float4 v = reinterpret_cast<const float4*>(src)[lane];
-        o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-        l = fmaf(src[129], f, l);
-      }
+  const int r = WARPS == 1 ? blockIdx.y * 8 + warp : blockIdx.y, rows = min(work.rows_tile, work.Sq * work.G - row0);
+  if (r >= rows) return;
+  // the parts of stream w0 + i: of its last slot for i = 0, its first for the others
+  const int n = cut.more + 1;
+  const int64_t step = static_cast<int64_t>(work.rows_tile) * 2 * kPartRow;
+  const float* base = parts + w0 * step + (static_cast<int64_t>(r / kRowTile) * 2 * kRowTile + r % kRowTile) * kPartRow;
+  auto part = [&](int i) { return base + i * step + (i == 0 ? cut.slot * (kRowTile * kPartRow) : 0); };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[128]);
+  m = warp_max(m);
+  const int i0 = WARPS == 1 ? 0 : static_cast<int>(static_cast<int64_t>(n) * warp / WARPS);
+  const int i1 = WARPS == 1 ? n : static_cast<int>(static_cast<int64_t>(n) * (warp + 1) / WARPS);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int at = i0; at < i1 && m != -INFINITY; at += 32) {
+    float f = 0.f;
+    if (at + lane < i1) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(at + lane) + 128);
+      f = fast_exp2(ml.x - m);
+      l = fmaf(ml.y, f, l);
     }
+    const int here = min(32, i1 - at);
+#pragma unroll 8
+    for (int k = 0; k < here; ++k) {
+      const float4 v = reinterpret_cast<const float4*>(part(at + k))[lane];
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      o.x = fmaf(v.x, fk, o.x), o.y = fmaf(v.y, fk, o.y), o.z = fmaf(v.z, fk, o.z), o.w = fmaf(v.w, fk, o.w);
+    }
+  }
+  l = warp_sum(l);
+  if constexpr (WARPS > 1) {
+    __shared__ float4 sums[WARPS][32];
+    __shared__ float lens[WARPS];
     sums[warp][lane] = o;
     if (lane == 0) lens[warp] = l;
     __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        const float4 v = sums[i][lane];
-        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-        l += lens[i];
-      }
-      const float inv = m == -INFINITY ? 0.f : 1.f / l;
-      uint2 u;
-      u.x = pack_bf16x2(o.x * inv, o.y * inv);
-      u.y = pack_bf16x2(o.z * inv, o.w * inv);
-      const int row = row0 + r, qi = work.by_G(row);
-      reinterpret_cast<uint2*>(p.o + b * p.o_sb + qi * p.o_ss + (cut.h * work.G + row - qi * work.G) * p.o_sh)[lane] = u;
+    if (warp > 0) return;
+    for (int i = 1; i < WARPS; ++i) {
+      const float4 v = sums[i][lane];
+      o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+      l += lens[i];
     }
-    __syncthreads();
   }
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  uint2 u;
+  u.x = pack_bf16x2(o.x * inv, o.y * inv);
+  u.y = pack_bf16x2(o.z * inv, o.w * inv);
+  const int row = row0 + r, qi = work.by_G(row);
+  reinterpret_cast<uint2*>(p.o + b * p.o_sb + qi * p.o_ss + (cut.h * work.G + row - qi * work.G) * p.o_sh)[lane] = u;
 }
 
 }  // namespace dsb
@@ -999,9 +1020,15 @@ extern "C" int dsb_kv_attn(const dsb_kv_cache* cache, const void* q, int64_t q_s
   cudaError_t err = launch_kernel(kern, static_cast<unsigned>(ctas), kAttnThreads, kAttnDynSmem, st, mk, mv, p, w, parts, cuts);
   if (err != cudaSuccess) return DSB_ERR_CUDA;
   if (cut && n_streams > 1) {
-    const int rows_cta = static_cast<int>(rows < 16 ? rows : 16);
-    err = launch_kernel(kv_combine_kernel, dim3(n_streams - 1, rows_cta), 256, 0, st, p, w, static_cast<const float*>(parts),
-                        static_cast<const KvCut*>(cuts));
+    const unsigned rows_item = static_cast<unsigned>(rows < w.rows_tile ? rows : w.rows_tile);
+    // parts of an item: about as many as there are streams for it.  One sequence of 131000 keys in 512 parts: 16 us with a warp
+    // for each row, 6 with 16.
+    if (n_streams > 32 * items)
+      err = launch_kernel(kv_combine_kernel<16>, dim3(static_cast<unsigned>(items), rows_item), 512, 0, st, p, w,
+                          static_cast<const float*>(parts), static_cast<const KvCut*>(cuts), n_streams);
+    else
+      err = launch_kernel(kv_combine_kernel<1>, dim3(n_streams - 1, (rows_item + 7) / 8), 256, 0, st, p, w,
+                          static_cast<const float*>(parts), static_cast<const KvCut*>(cuts), n_streams);
   }
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }

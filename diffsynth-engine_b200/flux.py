@@ -22,7 +22,7 @@ from typing import Dict, Optional
 
 import torch
 
-from . import ops
+from . import int4, ops
 from .packed import PackedLinear, act_format, pack_linear, stack_for_gemv
 
 
@@ -59,11 +59,16 @@ def sequence_slice(S_txt: int, S_img: int, world: int, rank: int) -> Dict[str, i
 class FluxDiTEngine:
     def __init__(self, state_dict: Dict[str, torch.Tensor], fmt: str = "fp8_tensor", device="cuda:0",
                  n_double: int = 19, n_single: int = 38, num_heads: int = 24, use_guidance: bool = True,
-                 release_source: bool = False, group=None):
+                 release_source: bool = False, group=None, mod_fmt: Optional[str] = None):
         """``group``: a ``torch.distributed`` process group to run the step sequence-parallel over (Ulysses): every
         rank then owns a contiguous slice of the joint text+image token sequence (padded to a multiple of the group
         size) for all token-wise kernels, and the joint attention exchanges heads for tokens; weights are
-        replicated (pass ``torch.distributed.group.WORLD`` for all ranks).  ``None`` = one GPU."""
+        replicated (pass ``torch.distributed.group.WORLD`` for all ranks).  ``None`` = one GPU.
+
+        ``mod_fmt``: format of the AdaLN modulation Linears (a quarter of the model's parameters, read once per step for one
+        conditioning vector); ``None`` = ``fmt``, ``"int4_group"`` = 4 bits with a scale and minimum for 32 columns."""
+        if mod_fmt not in (None, fmt, "int4_group"):
+            raise ValueError(f"mod_fmt must be None, '{fmt}' or 'int4_group', but got '{mod_fmt}'")
         from .wan import HeadExchange
         self.xchg = HeadExchange(group)
         # without a group the engine is a one-GPU replica even inside an initialised process group
@@ -102,11 +107,20 @@ class FluxDiTEngine:
             self.guid2 = P("guidance_embedder.timestep_embedder.2")
         self.pool0, self.pool2 = P("pooled_text_embedder.0"), P("pooled_text_embedder.2")
         self.ctx_emb, self.x_emb = P("context_embedder"), P("x_embedder")
+        def PM(name):   # a modulation Linear
+            if mod_fmt != "int4_group":
+                return P(name)
+            p = int4.pack_linear(sd[name + ".weight"], sd[name + ".bias"], self.dev)
+            if release_source:
+                sd.pop(name + ".weight", None)
+                sd.pop(name + ".bias", None)
+            return p
+
         mods = []
         self.double = []
         for i in range(n_double):
             pre = f"blocks.{i}."
-            mods += [P(pre + "norm1_a.linear"), P(pre + "norm1_b.linear")]
+            mods += [PM(pre + "norm1_a.linear"), PM(pre + "norm1_b.linear")]
             self.double.append(dict(
                 qkv_a=P(pre + "attn.a_to_qkv"), qkv_b=P(pre + "attn.b_to_qkv"),
                 nq_a=V(pre + "attn.norm_q_a.weight"), nk_a=V(pre + "attn.norm_k_a.weight"),
@@ -116,12 +130,12 @@ class FluxDiTEngine:
         self.single = []
         for i in range(n_single):
             pre = f"single_blocks.{i}."
-            mods.append(P(pre + "norm.linear"))
+            mods.append(PM(pre + "norm.linear"))
             self.single.append(dict(qkv_mlp=P(pre + "to_qkv_mlp"), nq=V(pre + "norm_q_a.weight"),
                                     nk=V(pre + "norm_k_a.weight"), proj=P(pre + "proj_out")))
-        mods.append(P("final_norm_out.linear"))
+        mods.append(PM("final_norm_out.linear"))
         self.final_proj = P("final_proj_out")
-        self.mod = stack_for_gemv(mods)
+        self.mod = int4.stack_for_gemv(mods) if mod_fmt == "int4_group" else stack_for_gemv(mods)
         del mods
         self._bufs = None
         self._graph = None
@@ -168,7 +182,10 @@ class FluxDiTEngine:
 
     # -------------------------------------------------------------------- pieces
     def _gemv(self, p: PackedLinear, x, out, act_in=ops.ACT_NONE, act_out=ops.ACT_NONE, accumulate=False):
-        ops.gemv(p.w, x, p.scale, p.bias, act_in=act_in, act_out=act_out, out=out, accumulate=accumulate)
+        if isinstance(p, int4.Int4Linear):
+            int4.gemv(p.w, x, p.bias, act_in=act_in, act_out=act_out, out=out, accumulate=accumulate)
+        else:
+            ops.gemv(p.w, x, p.scale, p.bias, act_in=act_in, act_out=act_out, out=out, accumulate=accumulate)
 
     def _quant(self, x, out, rs):
         """bf16 rows -> the GEMM's activation operand (+ per-row scale); a no-op view for bf16 weights."""

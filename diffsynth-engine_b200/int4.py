@@ -3,7 +3,8 @@
 codes; any other weight is quantised here.  A few activation rows are multiplied as they are (``dsb_gemv_int4``); for more rows
 the weight is expanded to bf16 (``dequant``) and goes through the GEMM."""
 import ctypes
-from typing import List
+from dataclasses import dataclass
+from typing import List, Optional
 
 import torch
 
@@ -14,6 +15,21 @@ from .ops import _ptr, _require_cuda, _rows, _stream
 GROUPS = (32, 64, 128)
 MAX_ROWS = 32     # DSB_INT4_MAX_ROWS: activation rows of one product
 GGUF_TYPES = ("Q4_0", "Q4_1", "Q4_K")
+
+
+@dataclass
+class Int4Linear:
+    """A 4-bit weight and its fp32 bias (``packed.PackedLinear`` of the other formats)."""
+    w: "Int4Weight"
+    bias: Optional[torch.Tensor]
+
+    @property
+    def out_features(self):
+        return self.w.N
+
+    @property
+    def in_features(self):
+        return self.w.K
 
 
 class Int4Weight:
@@ -146,6 +162,20 @@ def stack(parts: List[Int4Weight]) -> Int4Weight:
         raise _lib.DsbError("int4.stack: every part but the last has a multiple of 16 rows")
     return Int4Weight(torch.cat([p.payload for p in parts]), torch.cat([p.scales for p in parts]),
                       None if first.mins is None else torch.cat([p.mins for p in parts]), sum(p.N for p in parts), first.K, first.group)
+
+
+def pack_linear(weight, bias, device, group=32, asymmetric=True) -> Int4Linear:
+    """Quantises one ``[N, K]`` weight on the device."""
+    w = weight.reshape(weight.shape[0], -1).to(device=device)
+    if w.dtype not in (torch.float32, torch.bfloat16):
+        w = w.float()
+    b = None if bias is None else bias.to(device=device, dtype=torch.float32).contiguous()
+    return Int4Linear(quantize(w.contiguous(), group, asymmetric), b)
+
+
+def stack_for_gemv(parts: List[Int4Linear]) -> Int4Linear:
+    """Linears that share their input, as one (``packed.stack_for_gemv`` of the other formats)."""
+    return Int4Linear(stack([p.w for p in parts]), torch.cat([p.bias for p in parts]).contiguous())
 
 
 def dequant(w: Int4Weight, out=None):

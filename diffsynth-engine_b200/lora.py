@@ -151,11 +151,13 @@ def fuse_lora(module: torch.nn.Module) -> int:
     """For every ``LoRALinear``-like module below ``module`` (an ``nn.Linear`` with a ``_lora_dict`` of adapters
     carrying ``scale``/``alpha``/``rank``/``up``/``down``) whose weight was prepacked by ``enable_b200_linear``:
     route its forward through the fused path.  ``modify_scale``, ``add_lora`` and ``clear`` of the reference keep
-    working (the extension is rebuilt on the next call).  Returns the number of modules switched."""
-    from .quant import QuantLinearWeight
+    working (the extension is rebuilt on the next call).  Linears in 4 bits keep their adapters unfused.  Returns the number of
+    modules switched."""
+    from .quant import Int4LinearWeight, QuantLinearWeight
     n = 0
     for sub in module.modules():
         if isinstance(sub, torch.nn.Linear) and hasattr(sub, "_lora_dict") and isinstance(sub.weight, QuantLinearWeight) \
+                and not isinstance(sub.weight, Int4LinearWeight) \
                 and not getattr(type(sub), "_b200_fused_lora", False):
             cls = type(sub)
             sub.__class__ = type("B200Fused" + cls.__name__, (cls,), {"forward": _fused_forward,

@@ -11,6 +11,9 @@ weights that need metadata travel as a ``Parameter`` subclass (``GGUFParameter``
     with b200_inference():
         dit(...)                                      # every Linear whose weight is a QuantLinearWeight runs here
 
+``fmt="int4_group"`` keeps the weights in 4 bits with a scale and a minimum for 32 columns (``int4.py``): GGUF Q4_0, Q4_1 and Q4_K
+weights are taken over with their own codes, others are quantised.
+
 Anything that is not a ``QuantLinearWeight`` (VAE, text encoders, LoRA side matrices) falls through to the
 original ``F.linear`` untouched; ``lora.fuse_lora(dit)`` folds loaded-but-unfused LoRAs into the quantised GEMM.  Unlike the reference's context manager this one restores ``F.linear`` in a
 ``finally`` block.
@@ -21,8 +24,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import int4, ops
 from .packed import FORMATS, act_format
+
+LINEAR_FORMATS = FORMATS + ("int4_group",)
 
 
 class QuantLinearWeight(nn.Parameter):
@@ -53,6 +58,15 @@ class QuantLinearWeight(nn.Parameter):
         return self._bias_f32[1]
 
 
+class Int4LinearWeight(QuantLinearWeight):
+    """The payload of an ``int4.Int4Weight``; ``weight4`` is the whole of it."""
+
+    def __new__(cls, weight4: int4.Int4Weight):
+        self = QuantLinearWeight.__new__(cls, weight4.payload, None, "int4_group")
+        self.weight4 = weight4
+        return self
+
+
 def _gguf_type(weight):
     """The block format name ("Q8_0", "Q4_K", "Q6_K", ...) of a ``GGUFParameter`` (utils/gguf.py:9-59: raw uint8 rows
     plus a ``quant_dtype`` tag) if it is one this library dequantises itself - every format the reference does -
@@ -80,8 +94,14 @@ def _enable_b200_linear(module: nn.Module, fmt: str):
             raise ops._lib.DsbError("enable_b200_linear: move the module to the GPU first (no CPU path exists)")
         raw = raw.reshape(raw.shape[0], -1).contiguous()
         qt = _gguf_type(module.weight)
+        if fmt == "int4_group" and qt in int4.GGUF_TYPES:
+            module.weight = Int4LinearWeight(int4.from_gguf(raw, qt))
+            return
         w = (ops.dequant_q8_0(raw) if qt == "Q8_0" else ops.dequant_q4_k(raw) if qt == "Q4_K"
              else ops.dequant_gguf(raw, qt))
+        if fmt == "int4_group":
+            module.weight = Int4LinearWeight(int4.quantize(w, asymmetric=True))
+            return
         if fmt == "bf16":
             payload, scale = w, None
         else:
@@ -95,6 +115,9 @@ def _enable_b200_linear(module: nn.Module, fmt: str):
             raise ops._lib.DsbError("enable_b200_linear: move the module to the GPU first (no CPU path exists)")
         if w.dtype not in (torch.float32, torch.bfloat16):
             w = w.float()
+        if fmt == "int4_group":
+            module.weight = Int4LinearWeight(int4.quantize(w.contiguous(), asymmetric=True))
+            return
         if fmt == "bf16":
             payload, scale = w.to(torch.bfloat16).contiguous(), None
         else:
@@ -110,8 +133,8 @@ def enable_b200_linear(module: nn.Module, fmt: str = "fp8_tensor"):
     weight below ``module`` and mark the module.  GGUF Q8_0 and Q4_K weights (``GGUFParameter``) are dequantised once on the
     device (``fmt="bf16"`` keeps exactly the values the reference's ``gguf_linear`` multiplies with) and then take
     the same path, so they no longer depend on ``gguf_inference`` re-materialising them in every call."""
-    if fmt not in FORMATS:
-        raise ValueError(f"fmt must be one of {FORMATS}, but got '{fmt}'")
+    if fmt not in LINEAR_FORMATS:
+        raise ValueError(f"fmt must be one of {LINEAR_FORMATS}, but got '{fmt}'")
     _enable_b200_linear(module, fmt)
     setattr(module, "b200_linear_enabled", True)
 
@@ -123,12 +146,22 @@ def b200_linear(input: torch.Tensor, weight: torch.Tensor, bias=None, _origin=F.
         return _origin(input, weight, bias)
     if not input.is_cuda:
         raise ops._lib.DsbError("b200_linear got a CPU tensor: there is no CPU fallback")
-    N, K = weight.shape
+    w4 = weight.weight4 if isinstance(weight, Int4LinearWeight) else None
+    N, K = weight.shape if w4 is None else (w4.N, w4.K)
     x = input if input.dim() == 2 else input.reshape(-1, K)
     M = x.shape[0]
     b32 = weight.bias_f32(bias)
     ext = getattr(weight, "lora_ext", None)
-    if ext is None and M <= 4:
+    if w4 is not None:
+        if M <= int4.MAX_ROWS:
+            xf = x if x.dtype in (torch.bfloat16, torch.float32) else x.float()
+            y = int4.gemv(w4, xf if xf.stride(-1) == 1 and xf.stride(0) >= K else xf.contiguous(), b32)
+        else:
+            xb = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
+            if xb.stride(-1) != 1 or (xb.stride(0) % 8) or (xb.data_ptr() % 16):
+                xb = xb.contiguous()
+            y = ops.gemm(xb, int4.dequant(w4), bias=b32)
+    elif ext is None and M <= 4:
         # conditioning vectors: bandwidth-bound GEMV on fp32 activations, weights dequantised on the fly
         xf = x if x.dtype in (torch.bfloat16, torch.float32) else x.float()
         if xf.stride(-1) != 1:

@@ -31,7 +31,7 @@ from typing import Dict, Optional
 
 import torch
 
-from . import ops
+from . import kvcache, ops
 from .packed import PackedLinear, act_format, pack_linear
 
 
@@ -52,6 +52,7 @@ def wan_rope_table(f: int, h: int, w: int, head_dim: int = 128, theta: float = 1
     return torch.stack([torch.cos(ang), torch.sin(ang)], dim=-1).float().contiguous()
 
 
+CKV_PAGE = 64      # tokens per page of a prompt's keys and values in 8 bits
 IMG_TOKENS = 257   # CLIP tokens at the head of an image-to-video context (wan_dit.py:138-139)
 
 
@@ -110,7 +111,13 @@ class PeerMemory:
 class WanDiTEngine:
     def __init__(self, state_dict: Dict[str, torch.Tensor], fmt: str = "fp8_channel", device="cuda:0",
                  num_layers: int = 40, num_heads: int = 40, eps: float = 1e-6, freq_dim: int = 256, group=None,
-                 release_source: bool = False, overlap: bool = True, exchange: str = "auto", tail_split: bool = True):
+                 release_source: bool = False, overlap: bool = True, exchange: str = "auto", tail_split: bool = True,
+                 ckv_fmt: str = "bf16"):
+        """``ckv_fmt``: what the cross-attention keys and values of a prompt are kept in: "bf16" rows, or "e4m3" (a paged cache with
+        one power of two per 64 tokens and head: half the memory, read back to bf16 by the attention's own call)."""
+        if ckv_fmt not in ("bf16", "e4m3"):
+            raise ValueError(f"ckv_fmt must be 'bf16' or 'e4m3', but got '{ckv_fmt}'")
+        self.ckv_fmt = ckv_fmt
         self.dev = torch.device(device)
         self.fmt, self.afmt = fmt, act_format(fmt)
         self.L, self.H, self.eps, self.freq_dim = num_layers, num_heads, eps, freq_dim
@@ -268,7 +275,15 @@ class WanDiTEngine:
         b["ctx_rs"] = torch.zeros(L_all, dtype=f32, device=dev)
         # cross-attention keys and values of every block: they depend on the context only (wan_dit.py:143-149 applied to
         # the output of text_embedding), so they are computed once per prompt and reused by every later step
-        b["ckv"] = torch.zeros(max(self.L, 1), 2, L_all, d, dtype=bf, device=dev)
+        # (kept in 8 bits: one layer's rows on their way into the cache)
+        paged = self.ckv_fmt == "e4m3"
+        b["ckv"] = torch.zeros(1 if paged else max(self.L, 1), 2, L_all, d, dtype=bf, device=dev)
+        b["ckv8"] = None
+        if paged:
+            per = [-(-n // CKV_PAGE) for n in (ctx_len, n_img)]         # pages of a layer's text and image tokens
+            b["ckv8"] = kvcache.PagedKVCache.empty(max(self.L, 1) * sum(per), self.H, CKV_PAGE, dev)
+            pages = torch.arange(max(self.L, 1) * sum(per), dtype=torch.int32, device=dev).view(max(self.L, 1), 1, sum(per))
+            b["ckv8_txt"], b["ckv8_img"] = pages[:, :, :per[0]], pages[:, :, per[0]:]   # page tables, one per layer
         b["ctx_key"] = None
         if n_img:
             b["clip_in"] = torch.zeros(n_img, 1280, dtype=bf, device=dev)
@@ -378,16 +393,21 @@ class WanDiTEngine:
             cq_, cs_ = self._quant(b["ctx"], b["ctxq"][:, :d], b["ctx_rs"])    # quantised context, shared by all blocks
             cq_t, cs_t = cq_[txt_rows], (None if cs_ is None else cs_[txt_rows])
             for li, blk in enumerate(self.blocks):
-                ck_t, cv_t = ckv[li, 0, txt_rows], ckv[li, 1, txt_rows]
+                rows = ckv[li if b["ckv8"] is None else 0]
+                ck_t, cv_t = rows[0, txt_rows], rows[1, txt_rows]
                 self._gemm(cq_t, cs_t, blk["ck"], out=ck_t)
                 ops.rmsnorm_full(ck_t, blk["cnk"], None, 0, self.eps)
                 self._gemm(cq_t, cs_t, blk["cv"], out=cv_t)
                 if n_img:
                     cq_i, cs_i = cq_[:n_img], (None if cs_ is None else cs_[:n_img])
-                    ck_i, cv_i = ckv[li, 0, :n_img], ckv[li, 1, :n_img]
+                    ck_i, cv_i = rows[0, :n_img], rows[1, :n_img]
                     self._gemm(cq_i, cs_i, blk["ck_img"], out=ck_i)
                     ops.rmsnorm_full(ck_i, blk["cnk_img"], None, 0, self.eps)
                     self._gemm(cq_i, cs_i, blk["cv_img"], out=cv_i)
+                    if b["ckv8"] is not None:
+                        kvcache.append(b["ckv8"], ck_i.view(1, n_img, H, 128), cv_i.view(1, n_img, H, 128), b["ckv8_img"][li], 0)
+                if b["ckv8"] is not None:
+                    kvcache.append(b["ckv8"], ck_t.view(1, L, H, 128), cv_t.view(1, L, H, 128), b["ckv8_txt"][li], 0)
             b["ctx_valid"] = True
         # patch embedding: Conv3d with kernel = stride = (1,2,2) is a Linear over (c, y, z) patches (wan_dit.py:271-273)
         fr, gh, gw = b["grid"]
@@ -463,14 +483,17 @@ class WanDiTEngine:
             a, sc = self._ln(x, blk["n3_shift"], blk["n3_scale"], xq_d, rs[:Sl])
             self._gemm(a, sc, blk["cq"], out=proj[0])
             ops.rmsnorm_full(proj[0], blk["cnq"], None, 0, self.eps)
-            ck_t, cv_t = ckv[li, 0, txt_rows], ckv[li, 1, txt_rows]
-            ops.flash_attn(proj[0].view(1, Sl, H, 128), ck_t.view(1, L, H, 128), cv_t.view(1, L, H, 128),
-                           out=proj[1].view(1, Sl, H, 128))
+            def cross(rows, table, n, out):   # the queries over the n context rows of this layer
+                q4 = proj[0].view(1, Sl, H, 128)
+                if b["ckv8"] is None:
+                    ops.flash_attn(q4, ckv[li, 0, rows].view(1, n, H, 128), ckv[li, 1, rows].view(1, n, H, 128), out=out)
+                else:
+                    kvcache.attend(q4, b["ckv8"], table[li], n, out=out)
+
+            cross(txt_rows, b.get("ckv8_txt"), L, proj[1].view(1, Sl, H, 128))
             if n_img:   # the CLIP tokens have their own k/v projection; the two attention outputs add (wan_dit.py:147-151)
-                ck_i, cv_i = ckv[li, 0, :n_img], ckv[li, 1, :n_img]
                 att_i = qkv[:, :d]                                             # free until the next block's projection
-                ops.flash_attn(proj[0].view(1, Sl, H, 128), ck_i.view(1, n_img, H, 128), cv_i.view(1, n_img, H, 128),
-                               out=att_i.unflatten(1, (H, 128)).unsqueeze(0))
+                cross(slice(0, n_img), b.get("ckv8_img"), n_img, att_i.unflatten(1, (H, 128)).unsqueeze(0))
                 ops.gate_residual(proj[1], att_i, None, out=proj[1])           # bf16(x + y)
             a, sc = self._quant(proj[1], xq_d, rs[:Sl])
             self._gemm(a, sc, blk["co"], resid=x, out=x)

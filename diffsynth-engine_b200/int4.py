@@ -195,30 +195,41 @@ def gemv(w: Int4Weight, x, bias=None, act_in=ACT_NONE, act_out=ACT_NONE, out=Non
     """``act_out(act_in(x) @ w.T + bias)`` for one row ``x[K]`` or up to ``MAX_ROWS`` rows ``x[M, K]`` (float32 or bfloat16),
     fp32 arithmetic; ``out`` (default: the dtype of ``x``) is float32 or bfloat16 and, with ``accumulate``, added to."""
     _check_weight(w)
-    _require_cuda(x, bias, out)
-    N, K = w.N, w.K
-    one = x.dim() == 1
-    M, ld_x = (1, K) if one else (x.shape[0], x.stride(0))
-    if x.dim() > 2 or x.shape[-1] != K or x.stride(-1) != 1 or (M > 1 and ld_x < K):
-        raise _lib.DsbError(f"int4.gemv takes x as [{K}] or [M, {K}] with contiguous rows that do not overlap, got {tuple(x.shape)}")
+    dev, N, K = w._device, w.N, w.K
+    if x.get_device() != dev or (bias is not None and bias.get_device() != dev) or (out is not None and out.get_device() != dev):
+        _require_cuda(w.payload, x, bias, out)
+    shape, st = x.shape, x.stride()
+    if len(shape) == 2:
+        M, ld_x = shape[0], st[0]
+    elif len(shape) == 1:
+        M, ld_x = 1, K
+    else:
+        raise _lib.DsbError(f"int4.gemv takes x as [{K}] or [M, {K}], got {tuple(shape)}")
+    if shape[-1] != K or st[-1] != 1 or (M > 1 and ld_x < K):
+        raise _lib.DsbError(f"int4.gemv takes x as [{K}] or [M, {K}] with contiguous rows that do not overlap, got {tuple(shape)}")
     if M > MAX_ROWS:
         raise _lib.DsbError(f"int4.gemv takes up to {MAX_ROWS} rows, got {M}: expand the weight (int4.dequant) for more")
-    x_bf16 = x.dtype == torch.bfloat16
-    if not x_bf16 and x.dtype != torch.float32:
-        raise _lib.DsbError(f"int4.gemv takes float32 or bfloat16 rows, got {x.dtype}")
+    dtype = x.dtype
+    x_bf16 = dtype is torch.bfloat16
+    if not x_bf16 and dtype is not torch.float32:
+        raise _lib.DsbError(f"int4.gemv takes float32 or bfloat16 rows, got {dtype}")
     if out is None:
         if accumulate:
             raise _lib.DsbError("int4.gemv: accumulate needs an out to add to")
-        out, ld_y, y_bf16 = torch.empty((N,) if one else (M, N), dtype=x.dtype, device=x.device), N, x_bf16
+        out, ld_y, y_bf16 = x.new_empty((M, N) if len(shape) == 2 else (N,)), N, x_bf16
     else:
-        ld_y, y_bf16 = N if out.dim() == 1 else out.stride(0), out.dtype == torch.bfloat16
-        if out.dim() != x.dim() or tuple(out.shape) != ((N,) if one else (M, N)) or (out.stride(-1) != 1 and N > 1) or (M > 1 and ld_y < N):
-            raise _lib.DsbError(f"int4.gemv output must be {(N,) if one else (M, N)} with contiguous rows, got {tuple(out.shape)}")
-        if not y_bf16 and out.dtype != torch.float32:
+        want = (M, N) if len(shape) == 2 else (N,)
+        ld_y, y_bf16 = out.stride(0) if len(want) == 2 else N, out.dtype is torch.bfloat16
+        if out.shape != want or (out.stride(-1) != 1 and N > 1) or (M > 1 and ld_y < N):
+            raise _lib.DsbError(f"int4.gemv output must be {want} with contiguous rows, got {tuple(out.shape)}")
+        if not y_bf16 and out.dtype is not torch.float32:
             raise _lib.DsbError(f"int4.gemv writes float32 or bfloat16 rows, got {out.dtype}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
-        raise _lib.DsbError(f"int4.gemv bias must be contiguous float32 with {N} elements")
-    rc = _lib.lib().dsb_gemv_int4(w._ref, x.data_ptr(), ld_x, x_bf16, _ptr(bias), out.data_ptr(), ld_y, y_bf16, M, act_in, act_out,
+    bias_ptr = None
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.numel() != N or not bias.is_contiguous():
+            raise _lib.DsbError(f"int4.gemv bias must be contiguous float32 with {N} elements")
+        bias_ptr = bias.data_ptr()
+    rc = _lib.lib().dsb_gemv_int4(w._ref, x.data_ptr(), ld_x, x_bf16, bias_ptr, out.data_ptr(), ld_y, y_bf16, M, act_in, act_out,
                                   accumulate, _stream())
     check(rc, "dsb_gemv_int4")
     return out

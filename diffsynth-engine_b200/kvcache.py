@@ -72,23 +72,24 @@ def _here(cache, *ts):
 
 
 def _table(table, B):
-    if table.dtype != torch.int32 or table.dim() != 2:
+    shape, st = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(shape) != 2:
         raise _lib.DsbError(f"the page table is an int32 [{B}, pages] tensor with contiguous rows")
-    (rows, width), (ld, inner) = table.shape, table.stride()
+    (rows, width), (ld, inner) = shape, st
     if rows != B or width == 0 or (inner != 1 and width > 1) or (ld < width and B > 1):
         raise _lib.DsbError(f"the page table is an int32 [{B}, pages] tensor with contiguous rows")
     return (ld if ld > width else width), width
 
 
 def _per_sequence(t, B, what):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
         raise _lib.DsbError(f"{what} is an int or a contiguous int32 [{B}] tensor")
 
 
 def _rows4(t, what):
     """(shape, strides, address) of rows that the kernels take."""
     shape, st, ptr = t.shape, t.stride(), t.data_ptr()
-    if len(shape) != 4 or shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or st[3] != 1 or ptr % 16 \
+    if len(shape) != 4 or shape[3] != HEAD_DIM or t.dtype is not torch.bfloat16 or st[3] != 1 or ptr % 16 \
             or (st[0] | st[1] | st[2]) & 7 or st[0] < 0 or st[1] < 0 or st[2] < 0:
         raise _lib.DsbError(f"{what} is a bf16 [B, tokens, heads, 128] tensor with a contiguous head dimension, 16-byte aligned, "
                             "with strides that are multiples of 8")
@@ -184,8 +185,8 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     else:
         most = lens
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-        out_ptr, os = out.data_ptr(), out.stride()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_ptr, os = out.data_ptr(), (Sq * H * HEAD_DIM, H * HEAD_DIM, HEAD_DIM)
     else:
         out_shape, os, out_ptr = _rows4(out, "out")
         if out_shape != shape or any(st == 0 and n > 1 for st, n in zip(os, shape)):
@@ -201,7 +202,7 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     ws_ptr = ws_bytes = 0
     if most > UNCUT_TOKENS:         # a sequence may be cut along its keys
         ws_bytes = workspace_bytes(dev)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8)
         ws_ptr = ws.data_ptr()
     rc = _lib.lib().dsb_kv_attn(
         cache._ref, q_ptr, qs[0], qs[1], qs[2], out_ptr, os[0], os[1], os[2], B, Sq, H, table.data_ptr(), ld, width, _ptr(dev_lens), lens,

@@ -685,12 +685,12 @@ static int launch_gemv_int4(const Int4Dims& d, const GemvInt4& p, cudaStream_t s
   int n_share = d.row_blocks * 4 < 8 * sm_count() ? 8 : 4;
   while (n_share > 1 && d.k_tiles < 4 * n_share) n_share /= 2;
   if (d.row_blocks >= 16 * 8 * sm_count()) n_share = 1;
-  if (n_share == 1) {
-    const int rc = run_gemv_int4<NT, SPLIT, GROUP, MINS, false>(d, p, 1, st);
-    if (rc != DSB_ERR_UNSUPPORTED) return rc;
-    n_share = 8;
+  for (;;) {
+    const int rc = n_share == 1 ? run_gemv_int4<NT, SPLIT, GROUP, MINS, false>(d, p, 1, st)
+                                : run_gemv_int4<NT, SPLIT, GROUP, MINS, true>(d, p, n_share, st);
+    if (rc != DSB_ERR_UNSUPPORTED || n_share == 8) return rc;   // (a share that does not fit is cut further)
+    n_share *= 2;
   }
-  return run_gemv_int4<NT, SPLIT, GROUP, MINS, true>(d, p, n_share, st);
 }
 
 }  // namespace dsb
@@ -800,8 +800,8 @@ extern "C" int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // up to 16 columns of B at a time: 16 rows, or 8 of two columns each
   const bool split = !x_bf16 || act_in != DSB_ACT_NONE;
-  const int most = split ? 8 : 16;
-  for (int m0 = 0; m0 < M; m0 += most) {
+  int most = split ? 8 : 16;
+  for (int m0 = 0; m0 < M;) {
     GemvInt4 q = p;
     q.M = M - m0 < most ? M - m0 : most;
     q.x = reinterpret_cast<const uint8_t*>(x) + m0 * ld_x * (x_bf16 ? 2 : 4);
@@ -821,7 +821,12 @@ extern "C" int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld
     }
 #undef DSB_G4_GROUP
 #undef DSB_G4
+    if (rc == DSB_ERR_UNSUPPORTED && q.M > 1) {   // rows too long for so many at a time (nothing was launched)
+      most = (q.M + 1) / 2;
+      continue;
+    }
     if (rc != DSB_OK) return rc;
+    m0 += q.M;
   }
   return DSB_OK;
 }

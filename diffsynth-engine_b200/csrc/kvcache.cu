@@ -246,6 +246,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 __device__ __forceinline__ void e4m3x4_to_f16(uint32_t q, uint32_t& lo, uint32_t& hi) {
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(q));
 }
+// the four e4m3 values with zeros for NaN, which are noted
+__device__ __forceinline__ uint32_t e4m3_drop_nan(uint32_t q, uint32_t& nans) {
+  const uint32_t m = __vcmpeq4(q & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  nans |= m;
+  return q & ~m;
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -663,6 +669,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
       l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
     }
     // ---- O += P V: n tile n holds columns 16 g + n
+    uint32_t nans = 0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       uint4 w[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the half, chunk g
@@ -670,8 +677,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
       for (int x = 0; x < 4; ++x) {
         const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
         w[x] = *reinterpret_cast<const uint4*>(vs + key * kD + ((g ^ (key & 7)) << 4));
-        // behind the last key there may be anything, and 0 * NaN is NaN
-        if (!whole && (key0 + key >= ext || !(info1.x & (1 << hf)))) w[x] = make_uint4(0, 0, 0, 0);
+      }
+      if (!whole) {
+        // behind the last key there may be anything, and 0 * NaN is NaN; so it is for the rows that do not see a key yet
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
+          if (key0 + key >= ext || !(info1.x & (1 << hf))) w[x] = make_uint4(0, 0, 0, 0);
+          w[x].x = e4m3_drop_nan(w[x].x, nans), w[x].y = e4m3_drop_nan(w[x].y, nans);
+          w[x].z = e4m3_drop_nan(w[x].z, nans), w[x].w = e4m3_drop_nan(w[x].w, nans);
+        }
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -687,6 +702,27 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 4; ++e) mma_16816(o[4 * c + e], a[hf], b0[e], b1[e]);
       }
+    }
+    if (!whole && __any_sync(0xffffffffu, nans != 0)) {
+      // the NaN that were left out, for the rows that see them: columns 32 t + n of rows g and g + 8
+      uint32_t hit[2] = {0, 0};
+#pragma unroll 1
+      for (int key = 0; key < kTile; ++key) {
+        if (key0 + key >= ext || !(info1.x & (key < 16 ? 1 : 2))) continue;
+        uint32_t m = 0;
+#pragma unroll 1
+        for (int c = 0; c < 32; ++c) {
+          const uint32_t byte = vs[key * kD + (((2 * t + (c >> 4)) ^ (key & 7)) << 4) + (c & 15)];
+          m |= ((byte & 0x7fu) == 0x7fu ? 1u : 0u) << c;
+        }
+        hit[0] |= key0 + key < seen[0] ? m : 0;
+        hit[1] |= key0 + key < seen[1] ? m : 0;
+      }
+#pragma unroll
+      for (int n = 0; n < 16; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((hit[e >> 1] >> (n + 16 * (e & 1))) & 1u) o[n][e] = __int_as_float(0x7fffffff);
     }
     }
     __syncwarp();
@@ -708,7 +744,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
         if (row >= work.Sq * work.G) continue;
         // columns 32 t + n of the row are o[n][2 r], columns 32 t + 16 + n are o[n][2 r + 1]
         if (alone) {
-          const float inv = m_ref[r] == -INFINITY ? 0.f : 1.f / l_sum[r];
+          const float inv = l_sum[r] == 0.f ? 0.f : 1.f / l_sum[r];   // (no key: zeros; a row of NaN has no reference, but its sum is NaN)
           uint4* dst = reinterpret_cast<uint4*>(p.o + b * p.o_sb + qi * p.o_ss + (head * work.G + row - qi * work.G) * p.o_sh + 32 * t);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -729,7 +765,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<float4*>(dst + 32 * t + 16 * c + 4 * e) =
                   make_float4(o[4 * e][2 * r + c], o[4 * e + 1][2 * r + c], o[4 * e + 2][2 * r + c], o[4 * e + 3][2 * r + c]);
-          if (t == 0) dst[128] = m_ref[r], dst[129] = l_sum[r];
+          if (t == 0) dst[128] = m_ref[r] == -INFINITY && l_sum[r] != 0.f ? 0.f : m_ref[r], dst[129] = l_sum[r];
         }
       }
       if (parts && i + 1 == n_mine && sub == 0 && lane == 0) {

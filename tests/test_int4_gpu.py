@@ -135,6 +135,35 @@ def test_product_strides_activations_and_accumulation(dsb, cuda_dev):
     assert not bool(y[4][W[:, 9] != 0].isfinite().any())
 
 
+@pytest.mark.parametrize("M,K,dtype", [(1, 70002, torch.float32), (16, 70002, torch.bfloat16), (8, 120000, torch.float32)])
+def test_long_rows(dsb, cuda_dev, M, K, dtype):
+    """Rows that do not fit the shared memory of a CTA, or of a cluster, all at once."""
+    from diffsynth_engine_b200 import int4
+    c, s, m = _weight(33, K, 128, True, K)
+    w = int4.from_codes(*_on(cuda_dev, c, s, m), group=128)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dtype)
+    y = int4.gemv(w, x.to(cuda_dev), out=torch.empty(M, 33, device=cuda_dev))
+    assert O.rel_l2(y.cpu(), O4.linear(x, O4.values(c, s, m, 128))) < 4e-6        # (sixteen times the terms of the other shapes)
+
+
+def test_offsets_pass_32_bits(dsb, cuda_dev):
+    """2.5 GB of codes: rows at the end, and a dequantised row there."""
+    from diffsynth_engine_b200 import int4
+    N, K = 1200016, 4096
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=cuda_dev, dtype=torch.uint8)
+    scales = torch.rand(N, K // 64, generator=g, device=cuda_dev).half()
+    w = int4.from_codes(codes, scales, group=64)
+    x = torch.randn(1, K, generator=g, device=cuda_dev)
+    y = int4.gemv(w, x)[0]
+    for lo in (0, N // 2, N - 40):
+        ref = O4.linear(x.cpu(), O4.values(codes[lo:lo + 40].cpu(), scales[lo:lo + 40].cpu(), None, 64))[0]
+        assert O.rel_l2(y[lo:lo + 40].cpu(), ref) < 2e-6
+    del y
+    full = int4.dequant(w)
+    assert torch.equal(full[-3:].cpu(), O4.values(codes[-3:].cpu(), scales[-3:].cpu(), None, 64, torch.float32).bfloat16())
+
+
 def test_refusals(dsb, cuda_dev):
     from diffsynth_engine_b200 import int4
     c, s, m = _on(cuda_dev, *_weight(32, 64, 32, True, 0))

@@ -207,6 +207,69 @@ def test_blocks_of_very_different_scale(dsb, cuda_dev):
             assert O.rel_l2(out[0, i, h], ref[0, i, h]) < 2.0 ** -8 + 2.0 ** -10
 
 
+@pytest.mark.parametrize("T,n,Sq", [(16, 40, 20), (64, 100, 9), (64, 700, 5), (128, 1300, 40)])
+def test_nan_stays_with_the_rows_that_see_it(dsb, cuda_dev, T, n, Sq):
+    """A key, a value column or a query that is NaN reaches the rows that see it and no other; cut sequences too."""
+    from diffsynth_engine_b200 import kvcache
+    B, H, Hk = 2, 6, 2
+    W = -(-n // T) + 1
+    kv, ex = _pool(B * W, Hk, T, seed=T)
+    table = _table(B, W, B * W, seed=1)
+    q = torch.randn(B, Sq, H, 128, generator=torch.Generator().manual_seed(2)).bfloat16()
+
+    def put(i, b, tok, head, cols):
+        kv[i].view(torch.uint8)[int(table[b, tok // T]), head, tok % T, cols] = NAN8
+
+    put(1, 0, n - 2, 0, slice(17, 18))          # a value that the last two queries of sequence 0 see
+    put(0, 1, n - 3, 1, slice(5, 6))            # a key that the last three of sequence 1 see
+    q[0, 2, 5, 7] = float("nan")                # one row of its own
+    out = kvcache.attend(q.to(cuda_dev), _cache(cuda_dev, kv, ex), table.to(cuda_dev), torch.full((B,), n, dtype=torch.int32, device=cuda_dev),
+                         causal=True).cpu()
+    nan = out.isnan()
+    want = torch.zeros_like(nan)
+    want[0, Sq - 2:, :3, 17] = True
+    want[1, Sq - 3:, 3:] = True
+    want[0, 2, 5] = True
+    assert torch.equal(nan, want)
+    clean = [t.clone() for t in kv]
+    for t in clean:
+        t.view(torch.uint8)[t.view(torch.uint8) & 0x7f == 0x7f] = 0
+    q[0, 2, 5, 7] = 0
+    ref = OK.attend(q, [t.double() for t in clean], ex, table, [n] * B, True)
+    rows = ~want.any(-1)
+    assert O.rel_l2(out[rows], ref[rows]) < 2.0 ** -8 + 2.0 ** -11
+    keep = ~want[0, Sq - 2:, :3]
+    assert O.rel_l2(out[0, Sq - 2:, :3][keep], ref[0, Sq - 2:, :3][keep]) < 2.0 ** -8 + 2.0 ** -11
+
+
+def test_sequences_share_pages(dsb, cuda_dev):
+    """A prompt's pages, in the tables of several sequences."""
+    from diffsynth_engine_b200 import kvcache
+    kv, ex = _pool(8, 2, 32, seed=8)
+    table = torch.tensor([[3, 1, 4], [3, 1, 7], [3, 3, 3]], dtype=torch.int32)
+    q = torch.randn(3, 2, 4, 128, generator=torch.Generator().manual_seed(3)).bfloat16()
+    lens = [70, 96, 65]
+    out = kvcache.attend(q.to(cuda_dev), _cache(cuda_dev, kv, ex), table.to(cuda_dev), torch.tensor(lens, dtype=torch.int32, device=cuda_dev))
+    _near(out, OK.attend(q, [t.double() for t in kv], ex, table, lens), kv, ex)
+
+
+def test_pools_past_32_bits(dsb, cuda_dev):
+    """Pools of 5.4 GB each: appends, reads and attention on their last pages."""
+    from diffsynth_engine_b200 import kvcache
+    P, H, T = 41000, 8, 128
+    cache = kvcache.PagedKVCache.empty(P, H, T, cuda_dev)
+    table = torch.tensor([[P - 1, 5, P - 3]], dtype=torch.int32, device=cuda_dev)
+    g = torch.Generator(device=cuda_dev).manual_seed(0)
+    k, v = (torch.randn(1, 300, H, 128, generator=g, device=cuda_dev).bfloat16() for _ in range(2))
+    kvcache.append(cache, k, v, table, 0)
+    small = kvcache.PagedKVCache.empty(3, H, T, cuda_dev)
+    near = torch.tensor([[0, 1, 2]], dtype=torch.int32, device=cuda_dev)
+    kvcache.append(small, k, v, near, 0)
+    q = torch.randn(1, 4, 16, 128, generator=g, device=cuda_dev).bfloat16()
+    assert torch.equal(kvcache.attend(q, cache, table, 300, causal=True), kvcache.attend(q, small, near, 300, causal=True))
+    assert all(torch.equal(a, b) for a, b in zip(kvcache.read(cache, table, 300), kvcache.read(small, near, 300)))
+
+
 def test_bad_pages_and_lengths_are_masked_and_reported(dsb, cuda_dev):
     from diffsynth_engine_b200 import kvcache
     kv, ex = _pool(6, 2, 16, seed=4)

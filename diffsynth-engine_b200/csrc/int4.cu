@@ -43,29 +43,41 @@ __device__ __forceinline__ int64_t scale_index(const Int4Dims& d, int64_t row_bl
 }
 
 // ---------------------------------------------------------------------- layout
-// One thread per word of the payload.
+// One thread per lane of a tile: eight columns of two rows, twice.
 __global__ void __launch_bounds__(256) int4_pack_kernel(const uint8_t* __restrict__ codes, int64_t ld, Int4Dims d,
-                                                        uint32_t* __restrict__ payload) {
+                                                        uint4* __restrict__ payload) {
   grid_wait();
-  const int64_t total = static_cast<int64_t>(d.row_blocks) * d.k_tiles * 128;
+  const bool words = ((reinterpret_cast<uintptr_t>(codes) | ld) & 3) == 0;
+  const int64_t total = static_cast<int64_t>(d.row_blocks) * d.k_tiles * 32;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t tile = i >> 7;
-    const int lane = (i >> 2) & 31, j = i & 3, g = lane >> 2, t = lane & 3;
-    const int64_t rb = tile / d.k_tiles;
-    const int k = static_cast<int>(tile - rb * d.k_tiles) * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1);
-    uint32_t w = 0;
+    const int64_t tile = i >> 5, rb = tile / d.k_tiles;
+    const int lane = i & 31, g = lane >> 2, t = lane & 3, k0 = static_cast<int>(tile - rb * d.k_tiles) * 64 + 8 * t;
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int64_t row = rb * 16 + g + 8 * r;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t q = 8;
-        if (row < d.N && k + c < d.K) q = (codes[row * ld + ((k + c) >> 1)] >> (4 * (c & 1))) & 15u;
-        const int nibble = r + 2 * (c >> 1) + 4 * (c & 1);
-        w |= q << (4 * nibble);
+      for (int half = 0; half < 2; ++half) {
+        const int k = k0 + 32 * half;
+        uint32_t q = 0x88888888u;   // eight codes; those past the last column are 8
+        if (row < d.N && k < d.K) {
+          const uint8_t* at = codes + row * ld + (k >> 1);
+          if (words && k + 8 <= d.K) {
+            q = *reinterpret_cast<const uint32_t*>(at);
+          } else {
+            const int bytes = min(4, (d.K - k) >> 1);
+            for (int x = 0; x < bytes; ++x) q = (q & ~(255u << (8 * x))) | (static_cast<uint32_t>(at[x]) << (8 * x));
+          }
+        }
+        // columns c, c + 1, c + 2, c + 3 of a word go to nibbles r, r + 4, r + 2, r + 6
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t h = q >> (16 * j);
+          w[2 * half + j] |= ((h & 15u) | ((h >> 4 & 15u) << 16) | ((h >> 8 & 15u) << 8) | ((h >> 12 & 15u) << 24)) << (4 * r);
+        }
       }
     }
-    payload[i] = w;
+    payload[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -288,6 +300,14 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 // Split: a cluster of `n_share` CTAs owns a range of row blocks, each CTA a share of the columns, whose activations are all that
 // it stages; a warp takes every eighth row block of the range and streams its tiles without a pause from one to the next.
 // Shares meet in shared memory (CLUSTERED), in a fixed order.
+//
+// Bound by the bytes of the weight where there are many: 491520 x 5120 in groups of 32 takes 261 us (5.4 of 6.55 TB/s); 66
+// instructions for 512 bytes, 20 of them logic (one lop3 for two codes: written as and + or it is two, 292 us).  Small ones are
+// latency: 768 x 256 takes 3.4 us, 5120 x 5120 10.8 (2.5 at the copy rate): launch 2, activations 1.2, then a few batches of loads
+// and cold code, 1.6 for the two cluster barriers.  Tried and not kept: a cp.async ring instead of register buffers (342 us for the
+// large one), a third CTA per SM (80 registers: spills), each register slot refilled as it is used (the waits share scoreboards:
+// 622 with minima), equal runs of tiles for the warps instead of row blocks (+5 %), sums pushed into the owner's memory to save a
+// barrier (small 2.9, large 275).
 constexpr int kGemvSmemMax = 227 * 1024 - 1024;
 constexpr int kGemvCtas = 2;  // per SM
 constexpr int kBatch = 4;  // tiles of a warp in one of the two register buffers that the loads in flight fill
@@ -743,10 +763,10 @@ extern "C" int dsb_int4_pack(const uint8_t* codes, int64_t ld_codes, const void*
       !al(out_scales, 8) || !al(out_mins, 8) || !al(scales, 2) || !al(mins, 2))
     return DSB_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t words = static_cast<int64_t>(d.row_blocks) * d.k_tiles * 128;
+  const int64_t lanes = static_cast<int64_t>(d.row_blocks) * d.k_tiles * 32;
   const int64_t halves = static_cast<int64_t>(d.row_blocks) * d.scale_tiles * 16 * d.per_tile;
-  if (launch_kernel(int4_pack_kernel, stride_grid((words + 255) / 256), 256, 0, st, codes, ld_codes, d,
-                    reinterpret_cast<uint32_t*>(payload)) != cudaSuccess)
+  if (launch_kernel(int4_pack_kernel, stride_grid((lanes + 255) / 256), 256, 0, st, codes, ld_codes, d,
+                    reinterpret_cast<uint4*>(payload)) != cudaSuccess)
     return DSB_ERR_CUDA;
   const cudaError_t err = launch_kernel(int4_pack_scales_kernel, stride_grid((halves + 255) / 256), 256, 0, st,
                                         reinterpret_cast<const __half*>(scales), reinterpret_cast<const __half*>(mins), ld_scales, d,

@@ -53,15 +53,22 @@ struct KvAppend {
   int* status;
 };
 
-// One CTA per page that the rows of a sequence touch, head, and pool (k or v): its rows are read once, eight columns a load, kept
-// (rotated) in registers while the block's exponent is found, and written as e4m3.  CHUNKS: loads of a thread for a whole page.
-template <int THREADS, int CHUNKS>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(KvAppend p) {
+// A CTA has the rows that an append puts into one page of one pool (k or v), of some heads, one after the other: a head's rows are
+// read once, eight columns a load, and kept in registers (bf16) while the block's exponent is found, with the next head's on their
+// way.  The (cos, sin) of the rows are fetched once, into shared memory, and every key is rotated twice: for the exponent, and
+// to be written.  CHUNKS: loads of a thread for a whole page.
+//
+// Bound by the bytes: 256 in and 128 out for a row of a head.  Measured (us): 2 x about 4700 tokens of 40 heads, rotated, 68 (47 at
+// the copy rate); with a CTA for each head, rotations read from L2 by each and kept in fp32 registers, 83; the same with 256
+// threads a CTA 81 (pages of 64 tokens) to 131 (16); 512 tokens 5.3 against 7.3.  One token of 16 sequences: 3.1, latency.
+template <int THREADS, int CHUNKS, bool ROTATE>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constant__ KvAppend p, int heads_cta) {
   grid_wait();
-  __shared__ uint32_t red[THREADS / 32];
-  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, h = blockIdx.y, T = p.pool.T, tid = threadIdx.x;
+  extern __shared__ __align__(16) float4 turns[];   // ROTATE: [2 pairs of a float4][row][16]
+  __shared__ uint32_t red[2][THREADS / 32];
+  const int b = blockIdx.z >> 1, which = blockIdx.z & 1, T = p.pool.T, tid = threadIdx.x;
+  const int h0 = blockIdx.y * heads_cta, h1 = min(h0 + heads_cta, p.pool.heads);
   const int start = p.start ? p.start[b] : p.start_all, count = p.counts ? p.counts[b] : p.n;
-  const bool rotate = which == 0 && p.rope != nullptr;
   if (!kv_append_ok(start, count, p.n, p.tab.capacity(T)) ||
       (p.rope && count > 0 &&
        (start + static_cast<int64_t>(p.rope_row0) < 0 || start + static_cast<int64_t>(p.rope_row0) + count > p.rope_rows))) {
@@ -72,87 +79,148 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(KvAppend p) {
   if (s.rows == 0) return;
   const int page = kv_page(p.tab.row(b), p.tab.width, p.pool.n_pages, s.index);
   // (the rows are on their way while the page is looked up)
-  const __nv_bfloat16* src = p.src[which] + b * p.sb[which] + h * p.sh[which];
-  float x[CHUNKS][8];
-  uint32_t top = 0;   // largest finite magnitude, as bits
-  {
-    uint4 raw[CHUNKS];
+  const __nv_bfloat16* src = p.src[which] + b * p.sb[which] + static_cast<int64_t>(s.row) * p.sn[which];
+  const int chunks = s.rows * 16;
+  uint4 ahead[CHUNKS];
+  auto fetch = [&](int h) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       const int i = tid + c * THREADS;
-      raw[c] = make_uint4(0, 0, 0, 0);
-      if (i < s.rows * 16) {
-        const __nv_bfloat16* at = src + static_cast<int64_t>(s.row + (i >> 4)) * p.sn[which] + (i & 15) * 8;
+      ahead[c] = make_uint4(0, 0, 0, 0);
+      if (i < chunks) {
+        const __nv_bfloat16* at = src + h * p.sh[which] + (i >> 4) * p.sn[which] + (i & 15) * 8;
         asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w)
+                     : "=r"(ahead[c].x), "=r"(ahead[c].y), "=r"(ahead[c].z), "=r"(ahead[c].w)
                      : "l"(at));
       }
     }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      const int i = tid + c * THREADS;
-      const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 v = unpack_bf16x2(u[e]);
-        x[c][2 * e] = v.x, x[c][2 * e + 1] = v.y;
-      }
-      if (rotate && i < s.rows * 16) {
-        const float4* cs = reinterpret_cast<const float4*>(p.rope) +
-                           (static_cast<int64_t>(p.rope_row0) + start + s.row + (i >> 4)) * 32 + (i & 15) * 2;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float4 r = __ldg(cs + e);   // two pairs' (cos, sin)
-          float* v = x[c] + 4 * e;
-          const float a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
-          v[0] = __fsub_rn(__fmul_rn(a0, r.x), __fmul_rn(a1, r.y));
-          v[1] = __fadd_rn(__fmul_rn(a0, r.y), __fmul_rn(a1, r.x));
-          v[2] = __fsub_rn(__fmul_rn(a2, r.z), __fmul_rn(a3, r.w));
-          v[3] = __fadd_rn(__fmul_rn(a2, r.w), __fmul_rn(a3, r.z));
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t bits = __float_as_uint(x[c][e]) & 0x7fffffffu;
-        if (bits < 0x7f800000u) top = max(top, bits);
-      }
-    }
+  };
+  fetch(h0);
+  const bool rotate = ROTATE && which == 0;
+  if (rotate) {
+    const float4* cs = reinterpret_cast<const float4*>(p.rope) + (static_cast<int64_t>(p.rope_row0) + start + s.row) * 32;
+    for (int i = tid; i < s.rows * 32; i += THREADS) turns[(i & 1) * T * 16 + (i >> 1)] = __ldg(cs + i);
+    __syncthreads();
   }
   if (page < 0) {
     if (p.status) *p.status = DSB_ERR_ARG;
     return;
   }
-  const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
-  uint8_t* dst = (which ? p.pool.v : p.pool.k) + block * T * kD;
-  int8_t* exps = (which ? p.pool.v_exp : p.pool.k_exp) + block;
-  const int was = *exps;
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) red[tid >> 5] = top;
-  __syncthreads();
+  // columns 0..7 of a chunk in fp32, rotated where they are
+  auto values = [&](const uint4& w, int i, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) top = max(top, red[i]);
-  int e = kv_exponent(top);
-  if (s.slot > 0) {
-    e = max(e, was);
-    if (e > was) {
-      const float fall = pow2i(max(was - e, -126));   // (2^-127 and 2^-128 too take every e4m3 value to zero)
-      for (int i = tid; i < s.slot * (kD / 4); i += THREADS) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(dst) + i;
-        const uint32_t q = *at;
-        *at = e4m3x4(e4m3_to_float(q & 255u) * fall, e4m3_to_float((q >> 8) & 255u) * fall, e4m3_to_float((q >> 16) & 255u) * fall,
-                     e4m3_to_float(q >> 24) * fall);
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_bf16x2(u[e]);
+      v[2 * e] = f.x, v[2 * e + 1] = f.y;
+    }
+    if (rotate) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 r = turns[e * T * 16 + i];   // two pairs' (cos, sin)
+        float* x = v + 4 * e;
+        const float a0 = x[0], a1 = x[1], a2 = x[2], a3 = x[3];
+        x[0] = __fsub_rn(__fmul_rn(a0, r.x), __fmul_rn(a1, r.y));
+        x[1] = __fadd_rn(__fmul_rn(a0, r.y), __fmul_rn(a1, r.x));
+        x[2] = __fsub_rn(__fmul_rn(a2, r.z), __fmul_rn(a3, r.w));
+        x[3] = __fadd_rn(__fmul_rn(a2, r.w), __fmul_rn(a3, r.z));
       }
     }
-  }
-  if (tid == 0) *exps = static_cast<int8_t>(e);
-  const float inv = pow2i(-e);
+  };
+#pragma unroll 1
+  for (int h = h0; h < h1; ++h) {
+    const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
+    uint8_t* dst = (which ? p.pool.v : p.pool.k) + block * T * kD;
+    int8_t* exps = (which ? p.pool.v_exp : p.pool.k_exp) + block;
+    const int was = *exps;
+    uint4 raw[CHUNKS];
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int i = tid + c * THREADS;
-    if (i < s.rows * 16) {
-      const float* v = x[c];
+    for (int c = 0; c < CHUNKS; ++c) raw[c] = ahead[c];
+    if (h + 1 < h1) fetch(h + 1);
+    uint32_t top = 0;   // largest finite magnitude, as the bits of an fp32 number
+    if (rotate) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int i = tid + c * THREADS;
+        if (i >= chunks) break;
+        float v[8];
+        values(raw[c], i, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+          if (bits < 0x7f800000u) top = max(top, bits);
+        }
+      }
+    } else {
+      uint32_t most = 0;   // two bf16 magnitudes at a time
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t m = u[e] & 0x7fff7fffu;
+          most = __vmaxu2(most, m & __vcmpltu2(m, 0x7f807f80u));
+        }
+      }
+      top = max(most & 0xffffu, most >> 16) << 16;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((tid & 31) == 0) red[h & 1][tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) top = max(top, red[h & 1][i]);
+    int e = kv_exponent(top);
+    if (s.slot > 0) {
+      e = max(e, was);
+      if (e > was) {
+        const float fall = pow2i(max(was - e, -126));   // (2^-127 and 2^-128 too take every e4m3 value to zero)
+        for (int i = tid; i < s.slot * (kD / 4); i += THREADS) {
+          uint32_t* at = reinterpret_cast<uint32_t*>(dst) + i;
+          const uint32_t q = *at;
+          *at = e4m3x4(e4m3_to_float(q & 255u) * fall, e4m3_to_float((q >> 8) & 255u) * fall, e4m3_to_float((q >> 16) & 255u) * fall,
+                       e4m3_to_float(q >> 24) * fall);
+        }
+      }
+    }
+    if (tid == 0) *exps = static_cast<int8_t>(e);
+    const float inv = pow2i(-e);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = tid + c * THREADS;
+      if (i >= chunks) break;
+      float v[8];
+      values(raw[c], i, v);
       reinterpret_cast<uint2*>(dst + s.slot * kD)[i] =
           make_uint2(e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+    }
+  }
+}
+
+template <bool ROTATE>
+static cudaError_t launch_append(const KvAppend& p, cudaStream_t st) {
+  // heads of a CTA: one, until there are ten CTAs for every SM
+  const int64_t pages = static_cast<int64_t>(kv_span_pages(p.n, p.pool.T)) * p.B * 2, blocks = pages * p.pool.heads;
+  int heads = static_cast<int>(blocks / (10 * sm_count()));
+  heads = heads < 1 ? 1 : heads > p.pool.heads ? p.pool.heads : heads;
+  const dim3 grid(kv_span_pages(p.n, p.pool.T), (p.pool.heads + heads - 1) / heads, p.B * 2);
+  const size_t smem = ROTATE ? p.pool.T * 512 : 0;
+  switch (p.pool.T) {
+    case 16: return launch_kernel(kv_append_kernel<128, 2, ROTATE>, grid, 128, smem, st, p, heads);
+    case 32: return launch_kernel(kv_append_kernel<128, 4, ROTATE>, grid, 128, smem, st, p, heads);
+    case 64: return launch_kernel(kv_append_kernel<128, 8, ROTATE>, grid, 128, smem, st, p, heads);
+    default: {
+      auto kern = kv_append_kernel<256, 8, ROTATE>;   // (64 KB of rotations)
+      if (ROTATE) {
+        static std::atomic<unsigned long long> opted{0};
+        int dev = 0;
+        cudaError_t err = cudaGetDevice(&dev);
+        if (err != cudaSuccess) return err;
+        if (!(opted.load() >> (dev & 63) & 1)) {
+          if ((err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 512)) != cudaSuccess) return err;
+          opted.fetch_or(1ull << (dev & 63));
+        }
+      }
+      return launch_kernel(kern, grid, 256, smem, st, p, heads);
     }
   }
 }
@@ -167,7 +235,7 @@ struct KvRead {
   int* status;
 };
 
-// Eight lanes per (token, head) and pool, 16 columns each.  e4m3 * 2^e is exact in bf16 (but below 2^-126, where it is rounded).
+// Eight lanes per (token, head) and pool, 16 columns each; 1 byte read and 2 written for a value.  e4m3 * 2^e is exact in bf16 (but below 2^-126, where it is rounded).
 __global__ void __launch_bounds__(256) kv_read_kernel(KvRead p) {
   grid_wait();
   const int b = blockIdx.z >> 1, which = blockIdx.z & 1, T = p.pool.T, c = threadIdx.x & 7;
@@ -212,18 +280,28 @@ struct KvAttn {
   int* status;
 };
 
-// The rows (query, head of a group) of a sequence that share a cache head are taken 16 at a time; such a row tile, a cache head
-// and the keys that its rows see make an item, in tiles of 32 keys.  All tiles of all items, in order, are dealt out to the
-// warps of the grid in equal contiguous shares, whatever the lengths: a warp runs through its share without a pause, finishes the
-// items that are its own, and leaves partial results of the (at most two) items that it shares with others, which
-// kv_combine_kernel puts together in order.
+// The rows (query, head of a group) of a sequence that share a cache head are taken 16, 32 or 64 at a time (16 for each of up to four
+// warps); such a row tile, a cache head and the keys that its rows see make an item, in tiles of 32 keys.  All tiles of all items,
+// in order, are dealt out to the grid's streams in equal contiguous shares, whatever the lengths: a stream runs through its share
+// without a pause, finishes the items that are its own, and leaves partial results of the (at most two) items that it shares with
+// others, which kv_combine_kernel puts together in order.  Sequences of at most kMinShare tiles are not cut.
 //
-// Per warp: a ring of K and V tiles (TMA, 128-byte swizzle); S = Q K^T and O += P V with 16-bit tensor-core products and fp32
-// sums, fragments taken straight from the e4m3 bytes (exact in fp16).  Q is bf16 times a power of two per row, so exact in fp16
-// too but for values 2^-27 below the row's largest.  The scales: key j's score is t = S * c * 2^(ek + eq) + ev, in powers of two,
-// so that p = 2^(t - m) carries the value block's scale, and the row sum adds p * 2^-ev.  p is rounded to fp16: 11 bits, three
-// more than bf16 would keep.  The reference m of a row moves only when a score is 2^kSlack above it (p stays below 2^kSlack,
+// Per stream: a ring of K and V tiles (TMA, 128-byte swizzle); per warp S = Q K^T and O += P V with 16-bit tensor-core products and
+// fp32 sums, fragments taken straight from the e4m3 bytes (exact in fp16).  Q is bf16 times a power of two per row, so exact in
+// fp16 too but for values 2^-27 below the row's largest.  The scales: key j's score is t = S * c * 2^(ek + eq) + ev, in powers of
+// two, so that p = 2^(t - m) carries the value block's scale, and the row sum adds p * 2^-ev.  p is rounded to fp16: 11 bits,
+// three more than bf16 would keep.  The reference m of a row moves only when a score is 2^kSlack above it (p stays below 2^kSlack,
 // and fp16 has room to 2^16): moving it with every new maximum cost a rescaling of O in about every second tile.
+//
+// What bounds it: one row tile per cache head (a token of each sequence) the cache's bytes, behind about 10 us of start (lengths,
+// page table, first tiles, and code that no cache holds yet) and 4 for the combine pass.  A warp's tile takes about 2500 cycles
+// (S 780, softmax 560, P V 800, each a chain of dependent steps), and eight warps an SM are just what the memory rate needs; more
+// warps would halve the registers.  With more rows the same chains bind: 64 rows share a ring, but each warp converts for itself.
+// Measured (us): 77 keys x 24 heads 8; 16 ragged sequences of up to 16384 keys, 8 cache heads 70 (48 at the copy rate); 2 x 131071
+// keys, 32 rows 85 (32); 3 x 260 queries over ragged 8100 keys 456 (54 at the tensor rate of tcgen05, which mma.sync does not
+// reach).  Tried and slower: fragments of V made before the softmax and S in two sums (spills; 75 instead of 71), ten warps with
+// shorter rings (same; short calls +1), and converting each tile once for all its warps through shared memory, by warps of its own
+// (137 and 518 instead of 87 and 468) or by the consumers in parts (128 and 661).
 constexpr int kTile = 32;       // keys
 constexpr int kRowTile = 16;
 constexpr int kAttnWarps = 4;   // consumers per CTA
@@ -594,136 +672,139 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
     const uint8_t* vs = ks + kTile * kD;
     const bool whole = key0 + kTile <= all_see && info1.x == 3;
     if (key0 < any_see) {
-    // ---- scores: n tile j holds keys 8 j + g as columns
-    float s[4][4];
+      // ---- scores: n tile j holds keys 8 j + g as columns
+      float s[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 2; ++c) {
+        uint32_t u[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // chunk 2 t + c of the key's row lies at 2 t + c xor g (the swizzle): no two lanes of an eight share banks
-        const uint4 w = *reinterpret_cast<const uint4*>(ks + (8 * j + g) * kD + (((2 * t + c) ^ g) << 4));
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        for (int j = 0; j < 4; ++j) {
+          // chunk 2 t + c of the key's row lies at 2 t + c xor g (the swizzle): no two lanes of an eight share banks
+          const uint4 w = *reinterpret_cast<const uint4*>(ks + (8 * j + g) * kD + (((2 * t + c) ^ g) << 4));
+          u[j][0] = w.x, u[j][1] = w.y, u[j][2] = w.z, u[j][3] = w.w;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t b0, b1;
-          e4m3x4_to_f16(u[e], b0, b1);
-          mma_16816(s[j], q[c * 4 + e], b0, b1);
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            e4m3x4_to_f16(u[j][e], b0, b1);
+            mma_16816(s[j], q[c * 4 + e], b0, b1);
+          }
+      }
+      // ---- t = S c + ev, masked; the running reference
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float kf = pow2i(hf ? info1.z : info1.y), add = static_cast<float>(hf ? info2.x : info1.w);
+        const float f0 = c_row[0] * kf, f1 = c_row[1] * kf;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = 2 * hf + jj;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], e < 2 ? f0 : f1, add);
+          if (!whole) {
+            const bool there = info1.x & (1 << hf);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!there || key0 + 8 * j + 2 * t + (e & 1) >= seen[e >> 1]) s[j][e] = -INFINITY;
+          }
+          top[0] = max3f(top[0], s[j][0], s[j][1]);
+          top[1] = max3f(top[1], s[j][2], s[j][3]);
         }
       }
-    }
-    // ---- t = S c + ev, masked; the running reference
-    float top[2] = {-INFINITY, -INFINITY};
+      if (__any_sync(0xffffffffu, top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack)) {
+        float f[2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const float kf = pow2i(hf ? info1.z : info1.y), add = static_cast<float>(hf ? info2.x : info1.w);
-      const float f0 = c_row[0] * kf, f1 = c_row[1] * kf;
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const int j = 2 * hf + jj;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], e < 2 ? f0 : f1, add);
-        if (!whole) {
-          const bool there = info1.x & (1 << hf);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!there || key0 + 8 * j + 2 * t + (e & 1) >= seen[e >> 1]) s[j][e] = -INFINITY;
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          const bool moves = top[r] > m_ref[r] + kSlack;
+          f[r] = moves ? fast_exp2(m_ref[r] - top[r]) : 1.f;   // (0 for the first keys of a row)
+          m_ref[r] = moves ? top[r] : m_ref[r];
+          l_sum[r] *= f[r];
         }
-        top[0] = max3f(top[0], s[j][0], s[j][1]);
-        top[1] = max3f(top[1], s[j][2], s[j][3]);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
       }
-    }
-    if (__any_sync(0xffffffffu, top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack)) {
-      float f[2];
+      // (a row that has seen no key yet has no reference: its p are 2^-inf)
+      const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+      uint32_t a[2][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        const bool moves = top[r] > m_ref[r] + kSlack;
-        f[r] = moves ? fast_exp2(m_ref[r] - top[r]) : 1.f;   // (0 for the first keys of a row)
-        m_ref[r] = moves ? top[r] : m_ref[r];
-        l_sum[r] *= f[r];
+      for (int hf = 0; hf < 2; ++hf) {
+        const float inv_v = pow2i(-(hf ? info2.x : info1.w));
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = 2 * hf + jj;
+          s[j][0] = fast_exp2(s[j][0] - m0), s[j][1] = fast_exp2(s[j][1] - m0);
+          s[j][2] = fast_exp2(s[j][2] - m1), s[j][3] = fast_exp2(s[j][3] - m1);
+          sum0 += s[j][0] + s[j][1];
+          sum1 += s[j][2] + s[j][3];
+          a[hf][2 * jj] = pack_f16x2(s[j][0], s[j][1]);
+          a[hf][2 * jj + 1] = pack_f16x2(s[j][2], s[j][3]);
+        }
+        l_sum[0] = fmaf(sum0, inv_v, l_sum[0]);
+        l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
       }
+      // ---- O += P V: n tile n holds columns 16 g + n
+      uint32_t nans = 0;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
-    }
-    // (a row that has seen no key yet has no reference: its p are 2^-inf)
-    const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
-    uint32_t a[2][4];
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const float inv_v = pow2i(-(hf ? info2.x : info1.w));
-      float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const int j = 2 * hf + jj;
-        s[j][0] = fast_exp2(s[j][0] - m0), s[j][1] = fast_exp2(s[j][1] - m0);
-        s[j][2] = fast_exp2(s[j][2] - m1), s[j][3] = fast_exp2(s[j][3] - m1);
-        sum0 += s[j][0] + s[j][1];
-        sum1 += s[j][2] + s[j][3];
-        a[hf][2 * jj] = pack_f16x2(s[j][0], s[j][1]);
-        a[hf][2 * jj + 1] = pack_f16x2(s[j][2], s[j][3]);
-      }
-      l_sum[0] = fmaf(sum0, inv_v, l_sum[0]);
-      l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
-    }
-    // ---- O += P V: n tile n holds columns 16 g + n
-    uint32_t nans = 0;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      uint4 w[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the half, chunk g
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
-        w[x] = *reinterpret_cast<const uint4*>(vs + key * kD + ((g ^ (key & 7)) << 4));
-      }
-      if (!whole) {
-        // behind the last key there may be anything, and 0 * NaN is NaN; so it is for the rows that do not see a key yet
+      for (int hf = 0; hf < 2; ++hf) {
+        uint4 w[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the half, chunk g
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
-          if (key0 + key >= ext || !(info1.x & (1 << hf))) w[x] = make_uint4(0, 0, 0, 0);
-          w[x].x = e4m3_drop_nan(w[x].x, nans), w[x].y = e4m3_drop_nan(w[x].y, nans);
-          w[x].z = e4m3_drop_nan(w[x].z, nans), w[x].w = e4m3_drop_nan(w[x].w, nans);
+          w[x] = *reinterpret_cast<const uint4*>(vs + key * kD + ((g ^ (key & 7)) << 4));
+        }
+        if (!whole) {
+          // behind the last key there may be anything, and 0 * NaN is NaN; so it is for the rows that do not see a key yet
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
+            if (key0 + key >= ext || !(info1.x & (1 << hf))) w[x] = make_uint4(0, 0, 0, 0);
+            w[x].x = e4m3_drop_nan(w[x].x, nans), w[x].y = e4m3_drop_nan(w[x].y, nans);
+            w[x].z = e4m3_drop_nan(w[x].z, nans), w[x].w = e4m3_drop_nan(w[x].w, nans);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t v0 = c == 0 ? w[0].x : c == 1 ? w[0].y : c == 2 ? w[0].z : w[0].w;
+          const uint32_t v1 = c == 0 ? w[1].x : c == 1 ? w[1].y : c == 2 ? w[1].z : w[1].w;
+          const uint32_t v2 = c == 0 ? w[2].x : c == 1 ? w[2].y : c == 2 ? w[2].z : w[2].w;
+          const uint32_t v3 = c == 0 ? w[3].x : c == 1 ? w[3].y : c == 2 ? w[3].z : w[3].w;
+          uint32_t b0[4], b1[4];
+          e4m3x4_to_f16(__byte_perm(v0, v1, 0x5140), b0[0], b0[1]);
+          e4m3x4_to_f16(__byte_perm(v0, v1, 0x7362), b0[2], b0[3]);
+          e4m3x4_to_f16(__byte_perm(v2, v3, 0x5140), b1[0], b1[1]);
+          e4m3x4_to_f16(__byte_perm(v2, v3, 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mma_16816(o[4 * c + e], a[hf], b0[e], b1[e]);
         }
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t v0 = c == 0 ? w[0].x : c == 1 ? w[0].y : c == 2 ? w[0].z : w[0].w;
-        const uint32_t v1 = c == 0 ? w[1].x : c == 1 ? w[1].y : c == 2 ? w[1].z : w[1].w;
-        const uint32_t v2 = c == 0 ? w[2].x : c == 1 ? w[2].y : c == 2 ? w[2].z : w[2].w;
-        const uint32_t v3 = c == 0 ? w[3].x : c == 1 ? w[3].y : c == 2 ? w[3].z : w[3].w;
-        uint32_t b0[4], b1[4];
-        e4m3x4_to_f16(__byte_perm(v0, v1, 0x5140), b0[0], b0[1]);
-        e4m3x4_to_f16(__byte_perm(v0, v1, 0x7362), b0[2], b0[3]);
-        e4m3x4_to_f16(__byte_perm(v2, v3, 0x5140), b1[0], b1[1]);
-        e4m3x4_to_f16(__byte_perm(v2, v3, 0x7362), b1[2], b1[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mma_16816(o[4 * c + e], a[hf], b0[e], b1[e]);
-      }
-    }
-    if (!whole && __any_sync(0xffffffffu, nans != 0)) {
-      // the NaN that were left out, for the rows that see them: columns 32 t + n of rows g and g + 8
-      uint32_t hit[2] = {0, 0};
+      if (!whole && __any_sync(0xffffffffu, nans != 0)) {
+        // the NaN that were left out, for the rows that see them: columns 32 t + n of rows g and g + 8
+        uint32_t hit[2] = {0, 0};
 #pragma unroll 1
-      for (int key = 0; key < kTile; ++key) {
-        if (key0 + key >= ext || !(info1.x & (key < 16 ? 1 : 2))) continue;
-        uint32_t m = 0;
+        for (int key = 0; key < kTile; ++key) {
+          if (key0 + key >= ext || !(info1.x & (key < 16 ? 1 : 2))) continue;
+          uint32_t m = 0;
 #pragma unroll 1
-        for (int c = 0; c < 32; ++c) {
-          const uint32_t byte = vs[key * kD + (((2 * t + (c >> 4)) ^ (key & 7)) << 4) + (c & 15)];
-          m |= ((byte & 0x7fu) == 0x7fu ? 1u : 0u) << c;
+          for (int c = 0; c < 32; ++c) {
+            const uint32_t byte = vs[key * kD + (((2 * t + (c >> 4)) ^ (key & 7)) << 4) + (c & 15)];
+            m |= ((byte & 0x7fu) == 0x7fu ? 1u : 0u) << c;
+          }
+          hit[0] |= key0 + key < seen[0] ? m : 0;
+          hit[1] |= key0 + key < seen[1] ? m : 0;
         }
-        hit[0] |= key0 + key < seen[0] ? m : 0;
-        hit[1] |= key0 + key < seen[1] ? m : 0;
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((hit[e >> 1] >> (n + 16 * (e & 1))) & 1u) o[n][e] = __int_as_float(0x7fffffff);
       }
-#pragma unroll
-      for (int n = 0; n < 16; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((hit[e >> 1] >> (n + 16 * (e & 1))) & 1u) o[n][e] = __int_as_float(0x7fffffff);
-    }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[st][stage]);
@@ -914,15 +995,8 @@ extern "C" int dsb_kv_append(const dsb_kv_cache* cache, const void* k, int64_t k
   p.rope_rows = rope_rows;
   p.rope_row0 = rope_row0;
   p.status = status;
-  const dim3 grid(kv_span_pages(n, T), p.pool.heads, B * 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t err;
-  switch (T) {
-    case 16: err = launch_kernel(kv_append_kernel<128, 2>, grid, 128, 0, st, p); break;
-    case 32: err = launch_kernel(kv_append_kernel<128, 4>, grid, 128, 0, st, p); break;
-    case 64: err = launch_kernel(kv_append_kernel<128, 8>, grid, 128, 0, st, p); break;
-    default: err = launch_kernel(kv_append_kernel<256, 8>, grid, 256, 0, st, p); break;
-  }
+  const cudaError_t err = rope ? launch_append<true>(p, st) : launch_append<false>(p, st);
   return err == cudaSuccess ? DSB_OK : DSB_ERR_CUDA;
 }
 

@@ -4,6 +4,8 @@
 // steps), and the values themselves in 16 bits, so the attention multiplies what the cache stands for and nothing else.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "dsb.h"
 #include "kv_index.h"
@@ -58,14 +60,15 @@ struct KvAppend {
 // way.  The (cos, sin) of the rows are fetched once, into shared memory, and every key is rotated twice: for the exponent, and
 // to be written.  CHUNKS: loads of a thread for a whole page.
 //
-// Bound by the bytes: 256 in and 128 out for a row of a head.  Measured (us): 2 x about 4700 tokens of 40 heads, rotated, 68 (47 at
+// Bound by the bytes: 256 in and 128 out for a row of a head.  Measured (us): 2 x about 4700 tokens of 40 heads, rotated, 62 (47 at
 // the copy rate); with a CTA for each head, rotations read from L2 by each and kept in fp32 registers, 83; the same with 256
-// threads a CTA 81 (pages of 64 tokens) to 131 (16); 512 tokens 5.3 against 7.3.  One token of 16 sequences: 3.1, latency.
+// threads a CTA 81 (pages of 64 tokens) to 131 (16); with each magnitude compared with infinity 69.  512 tokens 5 to 7, one token of
+// 16 sequences 3: latency.
 template <int THREADS, int CHUNKS, bool ROTATE>
 __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constant__ KvAppend p, int heads_cta) {
   grid_wait();
   extern __shared__ __align__(16) float4 turns[];   // ROTATE: [2 pairs of a float4][row][16]
-  __shared__ uint32_t red[2][THREADS / 32];
+  __shared__ uint32_t red[2][THREADS / 32], red_finite[THREADS / 32];
   const int b = blockIdx.z >> 1, which = blockIdx.z & 1, T = p.pool.T, tid = threadIdx.x;
   const int h0 = blockIdx.y * heads_cta, h1 = min(h0 + heads_cta, p.pool.heads);
   const int start = p.start ? p.start[b] : p.start_all, count = p.counts ? p.counts[b] : p.n;
@@ -137,38 +140,44 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constan
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) raw[c] = ahead[c];
     if (h + 1 < h1) fetch(h + 1);
-    uint32_t top = 0;   // largest finite magnitude, as the bits of an fp32 number
-    if (rotate) {
+    // the CTA's largest magnitude, as the bits of an fp32 number; FINITE leaves out what is not (NaN is left out anyway)
+    auto largest = [&](auto finite, uint32_t* warps) {
+      uint32_t top;
+      if (rotate) {
+        float m = 0.f;
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const int i = tid + c * THREADS;
-        if (i >= chunks) break;
-        float v[8];
-        values(raw[c], i, v);
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int i = tid + c * THREADS;
+          if (i >= chunks) break;
+          float v[8];
+          values(raw[c], i, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
-          if (bits < 0x7f800000u) top = max(top, bits);
+          for (int e = 0; e < 8; ++e)
+            if (!finite.value || fabsf(v[e]) < INFINITY) m = fmaxf(m, fabsf(v[e]));
         }
-      }
-    } else {
-      uint32_t most = 0;   // two bf16 magnitudes at a time
+        top = __float_as_uint(m);
+      } else {
+        uint32_t most = 0;   // two bf16 magnitudes at a time
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+        for (int c = 0; c < CHUNKS; ++c) {
+          const uint32_t u[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t m = u[e] & 0x7fff7fffu;
-          most = __vmaxu2(most, m & __vcmpltu2(m, 0x7f807f80u));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t m = u[e] & 0x7fff7fffu;
+            most = __vmaxu2(most, finite.value ? m & __vcmpltu2(m, 0x7f807f80u) : m);
+          }
         }
+        top = max(most & 0xffffu, most >> 16) << 16;
       }
-      top = max(most & 0xffffu, most >> 16) << 16;
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((tid & 31) == 0) red[h & 1][tid >> 5] = top;
-    __syncthreads();
+      top = __reduce_max_sync(0xffffffffu, top);
+      if ((tid & 31) == 0) warps[tid >> 5] = top;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) top = max(top, red[h & 1][i]);
+      for (int i = 0; i < THREADS / 32; ++i) top = max(top, warps[i]);
+      return top;
+    };
+    uint32_t top = largest(std::false_type{}, red[h & 1]);
+    if (top >= 0x7f800000u) top = largest(std::true_type{}, red_finite);   // (the same for the whole CTA)
     int e = kv_exponent(top);
     if (s.slot > 0) {
       e = max(e, was);

@@ -13,8 +13,7 @@ from .ops import _ptr, _require_cuda, _stream, status_word
 HEAD_DIM = 128
 _SM_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 UNCUT_TOKENS = 256     # sequences up to this length are never cut (DSB_KV_UNCUT_TOKENS): no workspace
-# Queries from which on a length that the caller knows is worth bf16 rows of the whole sequence and the dense attention kernel
-DENSE_QUERIES = 256
+DENSE_QUERIES = 256    # fewer queries of a sequence always read the pages
 PAGE_TOKENS = (16, 32, 64, 128)
 
 
@@ -163,6 +162,21 @@ def workspace_bytes(device: int) -> int:
     return n
 
 
+def dense_pays(batch: int, queries: int, heads: int, cache_heads: int, tokens: int) -> bool:
+    """Whether ``attend`` gathers the sequences as bf16 rows for the dense attention kernel, instead of reading the pages: an estimate
+    of both in microseconds.  Pages: 9, 9 more where sequences may be cut, and 210 Mflop a microsecond.  Dense: the gather, then for
+    each query head of a group one launch of items of 256 rows, 74 at a time, each 2.4 and 0.62 a tile of 128 keys.  Measured
+    (pages, dense; heads / cache heads, queries x tokens): 24/24 256 x 77: 9, 13; 256 x 512: 24, 16; 4096 x 4096: 925, 190; 32/8
+    512 x 512: 38, 45; 4096 x 77: 50, 51; 4096 x 4096: 1228, 251; 4/1 1200 x 4096: 60, 132; 32760 x 512: 195, 66."""
+    if queries < DENSE_QUERIES or tokens <= 0 or batch <= 0:
+        return False
+    share = heads // cache_heads
+    pages = (9 if tokens <= UNCUT_TOKENS else 18) + 4 * HEAD_DIM * batch * queries * heads * (tokens + 64) / 210e6
+    waves = max(1.0, batch * cache_heads * -(-queries // 256) / 74)
+    dense = 5 + batch * tokens * cache_heads * 768 / 4e6 + share * (5 + waves * (2.4 + 0.62 * -(-tokens // 128)))
+    return dense < pages
+
+
 def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=None, out=None):
     """Attention of ``q`` (bf16 ``[B, Sq, H, 128]``) over the first ``lens`` tokens (int, or int32 ``[B]``) of each sequence; H is a
     multiple of the cache's heads, query head h reads cache head ``h // (H // heads)``.  ``causal``: query i sees the keys up to
@@ -193,7 +207,7 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
             raise _lib.DsbError("out has the shape of q and a place for each of its values")
     if sm_scale is None:
         sm_scale = _SM_SCALE
-    if dev_lens is None and not causal and Sq >= DENSE_QUERIES and lens > 0 and B > 0:
+    if dev_lens is None and not causal and dense_pays(B, Sq, H, heads, lens):
         k, v = read(cache, table, lens)
         share = H // heads
         for g in range(share):      # a cache head's queries, one of its query heads at a time

@@ -178,6 +178,29 @@ def test_attention(dsb, cuda_dev, B, Sq, H, Hk, T, lens, causal, sharp):
     assert bool((into[:, :, H:] == 5).all())
 
 
+@pytest.mark.parametrize("B,Sq,H,Hk,T,n,dense", [(1, 400, 4, 4, 64, 300, True), (2, 2100, 2, 1, 16, 513, True), (1, 257, 6, 1, 32, 90, False),
+                                                 (1, 700, 8, 1, 64, 640, False), (3, 256, 2, 2, 128, 385, True)])
+def test_many_queries_by_either_route(dsb, cuda_dev, B, Sq, H, Hk, T, n, dense):
+    """A known length: read back for the dense kernel where that is estimated to be less, the pages otherwise.  The dense kernel
+    rounds a probability to bf16, at most 2^-8 of it: on a result at most 2^-8 of the largest value, on all of them half a step
+    (2^-8 / sqrt 3 rms) as often as the result's own rounding, together less than 2^-8."""
+    from diffsynth_engine_b200 import kvcache
+    assert kvcache.dense_pays(B, Sq, H, Hk, n) == dense
+    W = -(-n // T)
+    kv, ex = _pool(B * W + 1, Hk, T, seed=n)
+    table = _table(B, W, B * W + 1, seed=Sq)
+    q = torch.randn(B, Sq, H, 128, generator=torch.Generator().manual_seed(7)).bfloat16()
+    ref = OK.attend(q, [t.double() for t in kv], ex, table, [n] * B, False)
+    cache = _cache(cuda_dev, kv, ex)
+    out = torch.full((B, Sq, H + 1, 128), 5.0, dtype=torch.bfloat16, device=cuda_dev)
+    kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), n, out=out[:, :, :H])
+    assert bool((out[:, :, H:] == 5).all())
+    out = out[:, :, :H].double().cpu()
+    top = float((kv[1].double().abs().amax(dim=(2, 3)) * 2.0 ** ex[1].double()).max())
+    assert float(((out - ref).abs() - ref.abs() * 2.0 ** -8).max()) <= 2.0 ** -8 * top
+    assert O.rel_l2(out, ref) < 2.0 ** -8 + 2.0 ** -11
+
+
 def _near(out, ref, kv, ex):
     out = out.double().cpu()
     assert bool(out.isfinite().all())

@@ -157,3 +157,12 @@ def test_cpu_tensors_are_refused(dsb):
     for call in (lambda: kvcache.append(c, x, x, t, 0), lambda: kvcache.attend(x, c, t, 1), lambda: kvcache.read(c, t, 1)):
         with pytest.raises(dsb.DsbError):
             call()
+
+
+def test_which_attention_a_known_length_takes():
+    """The gather and the dense kernel pay for many rows of a head; single tokens, empty sequences and many launches over little don't."""
+    from diffsynth_engine_b200 import kvcache
+    for args, dense in (((64, 1, 32, 8, 4096), False), ((1, 255, 24, 24, 4096), False), ((0, 300, 24, 24, 4096), False),
+                        ((1, 300, 24, 24, 0), False), ((1, 4096, 24, 24, 4096), True), ((1, 4096, 32, 8, 4096), True),
+                        ((1, 512, 32, 8, 512), False), ((1, 300, 1, 1, 100000), False), ((1, 32760, 4, 1, 512), True)):
+        assert kvcache.dense_pays(*args) == dense, args

@@ -111,11 +111,12 @@ def test_flux_modulation_in_4_bits(dsb, cuda_dev, graph):
 
 
 @pytest.mark.parametrize("grid,image", [((3, 8, 10), False), ((3, 8, 10), True), ((3, 20, 24), True)])
-def test_wan_prompt_cache_in_8_bits(dsb, cuda_dev, grid, image):
+def test_wan_prompt_cache_in_8_bits(dsb, cuda_dev, monkeypatch, grid, image):
     """The engine with its prompt's keys and values in the 8-bit cache is the engine whose bf16 ones have been rounded like that:
     60 queries (attention over the pages) and 360 (dense attention over rows read back, bit for bit the same)."""
     from diffsynth_engine_b200 import kvcache
     from diffsynth_engine_b200.wan import WanDiTEngine
+    monkeypatch.setattr(kvcache, "dense_pays", lambda batch, queries, *sizes: queries >= kvcache.DENSE_QUERIES)
     L, H, d = 2, 2, 256
     more = dict(in_dim=36, has_image_input=True) if image else {}
     w = {k: v.bfloat16().float() for k, v in synth.make_state_dict(

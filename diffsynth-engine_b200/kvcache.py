@@ -181,7 +181,8 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     """Attention of ``q`` (bf16 ``[B, Sq, H, 128]``) over the first ``lens`` tokens (int, or int32 ``[B]``) of each sequence; H is a
     multiple of the cache's heads, query head h reads cache head ``h // (H // heads)``.  ``causal``: query i sees the keys up to
     position ``lens - Sq + i`` (the queries are the sequence's last tokens, already appended).  A query that sees no key gives
-    zeros."""
+    zeros.  Table entries that are no pages raise at the next ``ops.check_status``; until then their keys count as masked, or as
+    zeros where ``dense_pays``."""
     dev_lens = lens if isinstance(lens, torch.Tensor) else None
     dev = _here(cache, q, table, dev_lens, out)
     shape, qs, q_ptr = _rows4(q, "q")
@@ -207,7 +208,8 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
             raise _lib.DsbError("out has the shape of q and a place for each of its values")
     if sm_scale is None:
         sm_scale = _SM_SCALE
-    if dev_lens is None and not causal and dense_pays(B, Sq, H, heads, lens):
+    # (the dense kernel's tensor maps have no stride of 0)
+    if dev_lens is None and not causal and dense_pays(B, Sq, H, heads, lens) and qs[0] and qs[1] and qs[2] and os[0] and os[1] and os[2]:
         k, v = read(cache, table, lens)
         share = H // heads
         for g in range(share):      # a cache head's queries, one of its query heads at a time

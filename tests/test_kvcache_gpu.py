@@ -201,6 +201,18 @@ def test_many_queries_by_either_route(dsb, cuda_dev, B, Sq, H, Hk, T, n, dense):
     assert O.rel_l2(out, ref) < 2.0 ** -8 + 2.0 ** -11
 
 
+def test_broadcast_queries(dsb, cuda_dev, monkeypatch):
+    """Queries with a stride of 0 read the pages, where others would take the dense kernel."""
+    from diffsynth_engine_b200 import kvcache
+    kv, ex = _pool(9, 2, 64, seed=2)
+    table, cache = _table(2, 4, 9, 3), _cache(cuda_dev, kv, ex)
+    monkeypatch.setattr(kvcache, "dense_pays", lambda *sizes: True)
+    q = torch.randn(2, 600, 2, 128, generator=torch.Generator().manual_seed(5)).bfloat16().to(cuda_dev)
+    for x in (q[:1].expand(2, -1, -1, -1), q[:, :1].expand(-1, 600, -1, -1), q[:, :, :1].expand(-1, -1, 2, -1)):
+        out = kvcache.attend(x, cache, table.to(cuda_dev), 250)
+        _near(out, OK.attend(x.cpu(), [t.double() for t in kv], ex, table, [250, 250]), kv, ex)
+
+
 def _near(out, ref, kv, ex):
     out = out.double().cpu()
     assert bool(out.isfinite().all())

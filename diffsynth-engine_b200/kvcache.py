@@ -164,16 +164,17 @@ def workspace_bytes(device: int) -> int:
 
 def dense_pays(batch: int, queries: int, heads: int, cache_heads: int, tokens: int) -> bool:
     """Whether ``attend`` gathers the sequences as bf16 rows for the dense attention kernel, instead of reading the pages: an estimate
-    of both in microseconds.  Pages: 9, 9 more where sequences may be cut, and 210 Mflop a microsecond.  Dense: the gather, then for
-    each query head of a group one launch of items of 256 rows, 74 at a time, each 2.4 and 0.62 a tile of 128 keys.  Measured
-    (pages, dense; heads / cache heads, queries x tokens): 24/24 256 x 77: 9, 13; 256 x 512: 24, 16; 4096 x 4096: 925, 190; 32/8
-    512 x 512: 38, 45; 4096 x 77: 50, 51; 4096 x 4096: 1228, 251; 4/1 1200 x 4096: 60, 132; 32760 x 512: 195, 66."""
+    of both in microseconds.  Pages: 9, 9 more where sequences may be cut, and 210 Mflop a microsecond.  Dense: 8 for the gather (4
+    on the device, but two calls' arguments) and its bytes, then for each query head of a group one launch of items of 256 rows, 74 at
+    a time, each 2.4 and 0.62 a tile of 128 keys; one cache head's query heads are rows of one launch.  Measured on the device (pages,
+    dense; heads / cache heads, queries x tokens): 24/24 256 x 77: 9, 13; 256 x 512: 24, 16; 4096 x 4096: 925, 190; 32/8 512 x 512:
+    38, 45; 4096 x 77: 50, 51; 4096 x 4096: 1228, 251; 4/1 1200 x 77: 10, 12; 1200 x 4096: 61, 37; 24440 x 512: 149, 39."""
     if queries < DENSE_QUERIES or tokens <= 0 or batch <= 0:
         return False
     share = heads // cache_heads
     pages = (9 if tokens <= UNCUT_TOKENS else 18) + 4 * HEAD_DIM * batch * queries * heads * (tokens + 64) / 210e6
     waves = max(1.0, batch * cache_heads * -(-queries // 256) / 74)
-    dense = 5 + batch * tokens * cache_heads * 768 / 4e6 + share * (5 + waves * (2.4 + 0.62 * -(-tokens // 128)))
+    dense = 8 + batch * tokens * cache_heads * 768 / 4e6 + share * (5 + waves * (2.4 + 0.62 * -(-tokens // 128)))
     return dense < pages
 
 
@@ -209,12 +210,19 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     if sm_scale is None:
         sm_scale = _SM_SCALE
     # (the dense kernel's tensor maps have no stride of 0)
-    if dev_lens is None and not causal and dense_pays(B, Sq, H, heads, lens) and qs[0] and qs[1] and qs[2] and os[0] and os[1] and os[2]:
-        k, v = read(cache, table, lens)
-        share = H // heads
-        for g in range(share):      # a cache head's queries, one of its query heads at a time
-            ops.flash_attn(q[:, :, g::share], k, v, out=out[:, :, g::share], sm_scale=sm_scale)
-        return out
+    if dev_lens is None and not causal and qs[0] and qs[1] and qs[2] and os[0] and os[1] and os[2]:
+        share, rows, q_row, o_row = H // heads, Sq, qs[1], os[1]
+        if heads == 1 and q_row == share * qs[2] and o_row == share * os[2]:
+            share, rows, q_row, o_row = 1, Sq * share, qs[2], os[2]       # one cache head: its query heads are rows like any others
+        if dense_pays(B, rows, heads * share, heads, lens):
+            k, v = read(cache, table, lens)
+            sb, sn, sh, _ = k.stride()
+            for g in range(share):      # a cache head's queries, one of its query heads at a time
+                rc = _lib.lib().dsb_flash_attn(
+                    q_ptr + 2 * g * qs[2], k.data_ptr(), v.data_ptr(), out_ptr + 2 * g * os[2], B, heads, rows, lens, HEAD_DIM,
+                    qs[0], q_row, share * qs[2], sb, sn, sh, sb, sn, sh, os[0], o_row, share * os[2], sm_scale, _status_ptr(dev), _stream())
+                check(rc, "dsb_flash_attn")
+            return out
     ws_ptr = ws_bytes = 0
     if most > UNCUT_TOKENS:         # a sequence may be cut along its keys
         ws_bytes = workspace_bytes(dev)

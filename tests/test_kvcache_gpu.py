@@ -179,7 +179,8 @@ def test_attention(dsb, cuda_dev, B, Sq, H, Hk, T, lens, causal, sharp):
 
 
 @pytest.mark.parametrize("B,Sq,H,Hk,T,n,dense", [(1, 400, 4, 4, 64, 300, True), (2, 2100, 2, 1, 16, 513, True), (1, 257, 6, 1, 32, 90, False),
-                                                 (1, 700, 8, 1, 64, 640, False), (3, 256, 2, 2, 128, 385, True)])
+                                                 (1, 700, 8, 1, 64, 640, False), (3, 256, 2, 2, 128, 385, True),
+                                                 (2, 900, 5, 1, 32, 200, False)])
 def test_many_queries_by_either_route(dsb, cuda_dev, B, Sq, H, Hk, T, n, dense):
     """A known length: read back for the dense kernel where that is estimated to be less, the pages otherwise.  The dense kernel
     rounds a probability to bf16, at most 2^-8 of it: on a result at most 2^-8 of the largest value, on all of them half a step
@@ -195,10 +196,11 @@ def test_many_queries_by_either_route(dsb, cuda_dev, B, Sq, H, Hk, T, n, dense):
     out = torch.full((B, Sq, H + 1, 128), 5.0, dtype=torch.bfloat16, device=cuda_dev)
     kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), n, out=out[:, :, :H])
     assert bool((out[:, :, H:] == 5).all())
-    out = out[:, :, :H].double().cpu()
+    whole = kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), n)     # (one cache head: its query heads as rows of one launch)
     top = float((kv[1].double().abs().amax(dim=(2, 3)) * 2.0 ** ex[1].double()).max())
-    assert float(((out - ref).abs() - ref.abs() * 2.0 ** -8).max()) <= 2.0 ** -8 * top
-    assert O.rel_l2(out, ref) < 2.0 ** -8 + 2.0 ** -11
+    for got in (out[:, :, :H].double().cpu(), whole.double().cpu()):
+        assert float(((got - ref).abs() - ref.abs() * 2.0 ** -8).max()) <= 2.0 ** -8 * top
+        assert O.rel_l2(got, ref) < 2.0 ** -8 + 2.0 ** -11
 
 
 def test_broadcast_queries(dsb, cuda_dev, monkeypatch):

@@ -183,7 +183,8 @@ def attend(q, cache: PagedKVCache, table, lens, causal: bool = False, sm_scale=N
     multiple of the cache's heads, query head h reads cache head ``h // (H // heads)``.  ``causal``: query i sees the keys up to
     position ``lens - Sq + i`` (the queries are the sequence's last tokens, already appended).  A query that sees no key gives
     zeros.  Table entries that are no pages raise at the next ``ops.check_status``; until then their keys count as masked, or as
-    zeros where ``dense_pays``."""
+    zeros where ``dense_pays``, which also takes bf16 rows of the sequences (512 bytes a token and cache head) for the time of the
+    call; lengths in a tensor always read the pages."""
     dev_lens = lens if isinstance(lens, torch.Tensor) else None
     dev = _here(cache, q, table, dev_lens, out)
     shape, qs, q_ptr = _rows4(q, "q")

@@ -299,8 +299,12 @@ struct KvAttn {
 // fp32 sums, fragments taken straight from the e4m3 bytes (exact in fp16).  Q is bf16 times a power of two per row, so exact in
 // fp16 too but for values 2^-27 below the row's largest.  The scales: key j's score is t = S * c * 2^(ek + eq) + ev, in powers of
 // two, so that p = 2^(t - m) carries the value block's scale, and the row sum adds p * 2^-ev.  p is rounded to fp16: 11 bits,
-// three more than bf16 would keep.  The reference m of a row moves only when a score is 2^kSlack above it (p stays below 2^kSlack,
-// and fp16 has room to 2^16): moving it with every new maximum cost a rescaling of O in about every second tile.
+// three more than bf16 would keep, where it is between 2^-14 and 2^16.  So the reference m of a row is set 2^kStart below its largest t
+// and moves only when a t is 2^kHigh above it (moving it with every new maximum cost a rescaling of O in about every second tile), and
+// a tile whose largest p of a row is below 2^-kLow - a flat tail behind one large score, or values far smaller than another
+// block's - is multiplied apart: p relative to its own largest t, and P V brought to the row's scale and added to O in fp32.  What
+// rounding leaves out of a p is at most 2^-12 of it, or 2^-25 / 2^-kLow = 2^-15 of the largest p of its row and tile (of its half
+// of the tile, where the halves are of two pages).
 //
 // What bounds it: one row tile per cache head (a token of each sequence) the cache's bytes, behind about 10 us of start (lengths,
 // page table, first tiles, and code that no cache holds yet) and 4 for the combine pass.  A warp's tile takes about 2500 cycles
@@ -321,13 +325,23 @@ constexpr int kStageBytes = 2 * kTile * kD;
 constexpr int kAttnRing = kAttnWarps * kAttnStages * kStageBytes;
 constexpr int kAttnDynSmem = kAttnRing + 1024;
 constexpr int kMinShare = DSB_KV_UNCUT_TOKENS / kTile;  // tiles: fewer are not worth another warp
-constexpr float kSlack = 8.f;
+constexpr float kStart = 12.f, kHigh = 15.f, kLow = 10.f;
 constexpr int kPartRow = 132;   // floats of a partial row: 128 columns, reference exponent, sum, two unused
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 2^x for x down to -149: value exponents may be 128 apart, and what is 2^-128 of one block's scale is not nothing in its own
+__device__ __forceinline__ float exp2_far(float x) {
+  const float y = fast_exp2(0.5f * x);
+  return y * y;
 }
 // four e4m3 values as two pairs of fp16
 __device__ __forceinline__ void e4m3x4_to_f16(uint32_t q, uint32_t& lo, uint32_t& hi) {
@@ -704,7 +718,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
           }
       }
       // ---- t = S c + ev, masked; the running reference
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[2] = {-INFINITY, -INFINITY}, top_half[2];   // (of the first half too, where the second is of another page)
+      const float hi0 = m_ref[0] + kHigh, hi1 = m_ref[1] + kHigh, lo0 = m_ref[0] - kLow, lo1 = m_ref[1] - kLow;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const float kf = pow2i(hf ? info1.z : info1.y), add = static_cast<float>(hf ? info2.x : info1.w);
@@ -723,74 +738,143 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
           top[0] = max3f(top[0], s[j][0], s[j][1]);
           top[1] = max3f(top[1], s[j][2], s[j][3]);
         }
+        if (T16 && hf == 0) top_half[0] = top[0], top_half[1] = top[1], top[0] = top[1] = -INFINITY;
       }
-      if (__any_sync(0xffffffffu, top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack)) {
-        float f[2];
+      const float least0 = T16 ? fminf(top[0], top_half[0]) : top[0], least1 = T16 ? fminf(top[1], top_half[1]) : top[1];
+      if (T16) top[0] = fmaxf(top[0], top_half[0]), top[1] = fmaxf(top[1], top_half[1]);
+      bool apart = false;
+      if (__any_sync(0xffffffffu, top[0] > hi0 || top[1] > hi1 || least0 < lo0 || least1 < lo1)) {
+        bool moves[2], low = false;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-          const bool moves = top[r] > m_ref[r] + kSlack;
-          f[r] = moves ? fast_exp2(m_ref[r] - top[r]) : 1.f;   // (0 for the first keys of a row)
-          m_ref[r] = moves ? top[r] : m_ref[r];
-          l_sum[r] *= f[r];
+          moves[r] = top[r] > m_ref[r] + kHigh;
+        }
+        if (__any_sync(0xffffffffu, moves[0] || moves[1])) {
+          float f[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            f[r] = moves[r] ? exp2_far(m_ref[r] - (top[r] - kStart)) : 1.f;   // (0 for the first keys of a row)
+            m_ref[r] = moves[r] ? top[r] - kStart : m_ref[r];
+            l_sum[r] *= f[r];
+          }
+#pragma unroll
+          for (int n = 0; n < 16; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
         }
 #pragma unroll
-        for (int n = 0; n < 16; ++n) o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
+        for (int r = 0; r < 2; ++r) {
+          // the smaller of the halves' largest t, if the row sees both; else the one that it sees
+          float least = top[r];
+          if (T16) {
+            float h0 = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+            float h1 = fmaxf(fmaxf(s[2][2 * r], s[2][2 * r + 1]), fmaxf(s[3][2 * r], s[3][2 * r + 1]));
+            h0 = fmaxf(h0, __shfl_xor_sync(0xffffffffu, h0, 1)), h0 = fmaxf(h0, __shfl_xor_sync(0xffffffffu, h0, 2));
+            h1 = fmaxf(h1, __shfl_xor_sync(0xffffffffu, h1, 1)), h1 = fmaxf(h1, __shfl_xor_sync(0xffffffffu, h1, 2));
+            least = h0 == -INFINITY ? h1 : h1 == -INFINITY ? h0 : fminf(h0, h1);
+          }
+          low |= least > -INFINITY && least < m_ref[r] - kLow;
+        }
+        apart = __any_sync(0xffffffffu, low);
       }
-      // (a row that has seen no key yet has no reference: its p are 2^-inf)
-      const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
-      uint32_t a[2][4];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const float inv_v = pow2i(-(hf ? info2.x : info1.w));
-        float sum0 = 0.f, sum1 = 0.f;
+      // 2^(t - sub) of a half, rounded to fp16, and their sums
+      auto probabilities = [&](int hf, float sub0, float sub1, uint32_t (&a)[4], float& sum0, float& sum1) {
+        sum0 = sum1 = 0.f;
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
           const int j = 2 * hf + jj;
-          s[j][0] = fast_exp2(s[j][0] - m0), s[j][1] = fast_exp2(s[j][1] - m0);
-          s[j][2] = fast_exp2(s[j][2] - m1), s[j][3] = fast_exp2(s[j][3] - m1);
+          s[j][0] = fast_exp2(s[j][0] - sub0), s[j][1] = fast_exp2(s[j][1] - sub0);
+          s[j][2] = fast_exp2(s[j][2] - sub1), s[j][3] = fast_exp2(s[j][3] - sub1);
           sum0 += s[j][0] + s[j][1];
           sum1 += s[j][2] + s[j][3];
-          a[hf][2 * jj] = pack_f16x2(s[j][0], s[j][1]);
-          a[hf][2 * jj + 1] = pack_f16x2(s[j][2], s[j][3]);
+          a[2 * jj] = pack_f16x2(s[j][0], s[j][1]);
+          a[2 * jj + 1] = pack_f16x2(s[j][2], s[j][3]);
         }
-        l_sum[0] = fmaf(sum0, inv_v, l_sum[0]);
-        l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
-      }
-      // ---- O += P V: n tile n holds columns 16 g + n
+      };
+      // O += P V of a half (APART: P V times a number for each row): n tile n holds columns 16 g + n
       uint32_t nans = 0;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
+      auto products = [&](auto is_apart, int hf, const uint32_t (&a)[4], float unit0, float unit1) {
         uint4 w[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the half, chunk g
+        auto row = [&](int x) { const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1); return key; };
+        if constexpr (!is_apart.value) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
-          w[x] = *reinterpret_cast<const uint4*>(vs + key * kD + ((g ^ (key & 7)) << 4));
-        }
-        if (!whole) {
-          // behind the last key there may be anything, and 0 * NaN is NaN; so it is for the rows that do not see a key yet
+          for (int x = 0; x < 4; ++x) w[x] = *reinterpret_cast<const uint4*>(vs + row(x) * kD + ((g ^ (row(x) & 7)) << 4));
+          if (!whole) {
+            // behind the last key there may be anything, and 0 * NaN is NaN; so it is for the rows that do not see a key yet
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = 16 * hf + 2 * t + (x & 1) + 8 * (x >> 1);
-            if (key0 + key >= ext || !(info1.x & (1 << hf))) w[x] = make_uint4(0, 0, 0, 0);
-            w[x].x = e4m3_drop_nan(w[x].x, nans), w[x].y = e4m3_drop_nan(w[x].y, nans);
-            w[x].z = e4m3_drop_nan(w[x].z, nans), w[x].w = e4m3_drop_nan(w[x].w, nans);
+            for (int x = 0; x < 4; ++x) {
+              if (key0 + row(x) >= ext || !(info1.x & (1 << hf))) w[x] = make_uint4(0, 0, 0, 0);
+              w[x].x = e4m3_drop_nan(w[x].x, nans), w[x].y = e4m3_drop_nan(w[x].y, nans);
+              w[x].z = e4m3_drop_nan(w[x].z, nans), w[x].w = e4m3_drop_nan(w[x].w, nans);
+            }
           }
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t v0 = c == 0 ? w[0].x : c == 1 ? w[0].y : c == 2 ? w[0].z : w[0].w;
-          const uint32_t v1 = c == 0 ? w[1].x : c == 1 ? w[1].y : c == 2 ? w[1].z : w[1].w;
-          const uint32_t v2 = c == 0 ? w[2].x : c == 1 ? w[2].y : c == 2 ? w[2].z : w[2].w;
-          const uint32_t v3 = c == 0 ? w[3].x : c == 1 ? w[3].y : c == 2 ? w[3].z : w[3].w;
-          uint32_t b0[4], b1[4];
-          e4m3x4_to_f16(__byte_perm(v0, v1, 0x5140), b0[0], b0[1]);
-          e4m3x4_to_f16(__byte_perm(v0, v1, 0x7362), b0[2], b0[3]);
-          e4m3x4_to_f16(__byte_perm(v2, v3, 0x5140), b1[0], b1[1]);
-          e4m3x4_to_f16(__byte_perm(v2, v3, 0x7362), b1[2], b1[3]);
+          uint32_t v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma_16816(o[4 * c + e], a[hf], b0[e], b1[e]);
+          for (int x = 0; x < 4; ++x) {
+            if constexpr (is_apart.value) {   // (a word at a time and in order: ahead of their use they cost spills)
+              v[x] = *reinterpret_cast<const volatile uint32_t*>(vs + row(x) * kD + ((g ^ (row(x) & 7)) << 4) + 4 * c);
+              if (!whole) v[x] = e4m3_drop_nan(key0 + row(x) >= ext || !(info1.x & (1 << hf)) ? 0u : v[x], nans);
+            } else {
+              v[x] = c == 0 ? w[x].x : c == 1 ? w[x].y : c == 2 ? w[x].z : w[x].w;
+            }
+          }
+          uint32_t b0[4], b1[4];
+          e4m3x4_to_f16(__byte_perm(v[0], v[1], 0x5140), b0[0], b0[1]);
+          e4m3x4_to_f16(__byte_perm(v[0], v[1], 0x7362), b0[2], b0[3]);
+          e4m3x4_to_f16(__byte_perm(v[2], v[3], 0x5140), b1[0], b1[1]);
+          e4m3x4_to_f16(__byte_perm(v[2], v[3], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float(&to)[4] = o[4 * c + e];
+            if constexpr (is_apart.value) {
+              float x[4];
+              mma_16816_first(x, a, b0[e], b1[e]);
+              to[0] = fmaf(x[0], unit0, to[0]), to[1] = fmaf(x[1], unit0, to[1]);
+              to[2] = fmaf(x[2], unit1, to[2]), to[3] = fmaf(x[3], unit1, to[3]);
+            } else {
+              mma_16816(to, a, b0[e], b1[e]);
+            }
+          }
+        }
+      };
+      // (a row that has seen no key yet has no reference: its p are 2^-inf)
+      if (!apart) {
+        const float m0 = m_ref[0] == -INFINITY ? 0.f : m_ref[0], m1 = m_ref[1] == -INFINITY ? 0.f : m_ref[1];
+        uint32_t a[2][4];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float inv_v = pow2i(-(hf ? info2.x : info1.w));
+          float sum0, sum1;
+          probabilities(hf, m0, m1, a[hf], sum0, sum1);
+          l_sum[0] = fmaf(sum0, inv_v, l_sum[0]);
+          l_sum[1] = fmaf(sum1, inv_v, l_sum[1]);
+        }
+        products(std::false_type{}, 0, a[0], 1.f, 1.f);
+        products(std::false_type{}, 1, a[1], 1.f, 1.f);
+      } else {
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {   // (the half's scores are always s[0] and s[1])
+          const float ev = static_cast<float>(hf ? info2.x : info1.w);
+          float most[2], unit[2], sum[2];
+          uint32_t a[4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            most[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+            most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
+            most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
+            most[r] -= kStart;                                                 // (room below it, as for a row's reference)
+            unit[r] = most[r] == -INFINITY ? -INFINITY : most[r] - m_ref[r];   // (no key of the half: nothing to add)
+            most[r] = most[r] == -INFINITY ? 0.f : most[r];
+          }
+          probabilities(0, most[0], most[1], a, sum[0], sum[1]);
+          l_sum[0] = fmaf(sum[0], exp2_far(unit[0] - ev), l_sum[0]);
+          l_sum[1] = fmaf(sum[1], exp2_far(unit[1] - ev), l_sum[1]);
+          products(std::true_type{}, hf, a, exp2_far(unit[0]), exp2_far(unit[1]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][e] = s[2][e], s[1][e] = s[3][e];
         }
       }
       if (!whole && __any_sync(0xffffffffu, nans != 0)) {
@@ -910,7 +994,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) kv_combine_kern
     float f = 0.f;
     if (at + lane < i1) {
       const float2 ml = *reinterpret_cast<const float2*>(part(at + lane) + 128);
-      f = fast_exp2(ml.x - m);
+      f = exp2_far(ml.x - m);
       l = fmaf(ml.y, f, l);
     }
     const int here = min(32, i1 - at);

@@ -1,0 +1,115 @@
+"""Attention over the paged cache where its numbers lie far apart: value blocks of one sequence with very different exponents, one
+key far above a flat tail.
+
+Tolerance: the output is rounded to bf16 (2^-8 of a value at most, 2^-8 / sqrt 3 rms), and each probability to 11 bits (2^-11), as in
+test_kvcache_gpu: 2^-8 + 2^-11 of each row's own norm, and per value 2^-8 of it plus 2^-10 of the largest value that the row
+averages with any weight to speak of."""
+import pytest
+import torch
+
+from oracle import kvcache as OK
+from oracle import ops as O
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled(dev, B, Hk, T, lens, k, v, table):
+    from diffsynth_engine_b200 import kvcache
+    cache = kvcache.PagedKVCache.empty(int(table.max()) + 1, Hk, T, dev)
+    kvcache.append(cache, k.to(dev), v.to(dev), table.to(dev), 0, torch.tensor(lens, dtype=torch.int32, device=dev))
+    return cache
+
+
+def _held(cache):
+    return [cache.k.cpu().double(), cache.v.cpu().double()], [cache.k_exp.cpu(), cache.v_exp.cpu()]
+
+
+def _rows_near(out, ref, top):
+    out = out.double().cpu()
+    assert bool(out.isfinite().all())
+    for got, want in zip(out.reshape(-1, 128), ref.reshape(-1, 128)):
+        assert O.rel_l2(got, want) < 2.0 ** -8 + 2.0 ** -11
+        assert float(((got - want).abs() - want.abs() * 2.0 ** -8).max()) <= 2.0 ** -10 * top
+
+
+@pytest.mark.parametrize("T", [16, 64])
+@pytest.mark.parametrize("B,Sq,H,Hk,lens,causal", [(1, 1, 1, 1, [200], False), (2, 3, 8, 2, [256, 130], True), (1, 40, 4, 2, [230], False),
+                                                   (1, 2, 4, 2, [3000], False), (3, 1, 4, 4, [900, 1500, 33], True), (1, 70, 2, 1, [1200], True)])
+@pytest.mark.parametrize("big", [1e4, 1e6, 1e8, 1e18])
+def test_a_large_value_that_nobody_looks_at(dsb, cuda_dev, T, B, Sq, H, Hk, lens, causal, big):
+    """One token of a sequence has a large value and no weight: every row is an average of the values around 0.02."""
+    from diffsynth_engine_b200 import kvcache
+    W = -(-max(lens) // T)
+    table = torch.randperm(B * W, generator=torch.Generator().manual_seed(3)).view(B, W).int()
+    g = torch.Generator().manual_seed(T + Sq)
+    n = max(lens)
+    q, k = torch.randn(B, Sq, H, 128, generator=g), torch.randn(B, n, Hk, 128, generator=g)
+    v = (torch.randn(B, n, Hk, 128, generator=g) * 0.005 + 0.02)
+    q[..., 0] = 30.0
+    k[..., 0] = 0.0
+    k[:, 21, :, 0] = -300.0              # a score of about -800: its weight is 0 in any arithmetic
+    v[:, 21] *= big
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    cache = _filled(cuda_dev, B, Hk, T, lens, k, v, table)
+    kv, ex = _held(cache)
+    ref = OK.attend(q, kv, ex, table, lens, causal)
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    top = 0.05                           # (the largest of the values that have a weight)
+    out = kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), lt, causal=causal)
+    _rows_near(out, ref, top)
+    assert torch.equal(out, kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), lt, causal=causal))
+
+
+@pytest.mark.parametrize("exps", [[-64, 64, -64, 64, -64, 64, -64, 64], [64, -64, -64, -64, -64, -64, -64, -64], [-64] * 7 + [64], [0, -30, 20, -64, 64, 3, -3, 12]])
+@pytest.mark.parametrize("T,copies", [(16, 1), (32, 1), (64, 1), (16, 20), (64, 12)])
+def test_weight_on_blocks_of_any_exponent(dsb, cuda_dev, exps, T, copies):
+    """Query i looks at the keys of every eighth page from i on, evenly: it gets their values with their own precision, whatever the others hold."""
+    from diffsynth_engine_b200 import kvcache
+    P = 8
+    g = torch.Generator().manual_seed(T)
+    v = (torch.rand(P, 2, T, 128, generator=g) * 200 + 200).to(torch.float8_e4m3fn)
+    k = torch.zeros(P, 2, T, 128)
+    for j in range(P):
+        k[j, :, :, j] = 16.0
+    q = torch.zeros(1, P, 4, 128)
+    for i in range(P):
+        q[0, i, :, i] = 60.0            # a score of 960 against 0: the other pages have no weight
+    k, q = k.to(torch.float8_e4m3fn), q.bfloat16()
+    ex = [torch.zeros(P, 2, dtype=torch.int8), torch.tensor(exps, dtype=torch.int8)[:, None].repeat(1, 2).contiguous()]
+    cache = kvcache.PagedKVCache(k.to(cuda_dev), v.to(cuda_dev), *(e.to(cuda_dev) for e in ex))
+    table = torch.arange(P, dtype=torch.int32).repeat(copies)[None].contiguous()
+    n = P * T * copies
+    ref = OK.attend(q, [k.double(), v.double()], ex, table, [n], sm_scale=1.0)
+    out = kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), torch.tensor([n], dtype=torch.int32, device=cuda_dev), sm_scale=1.0)
+    for i in range(P):
+        _rows_near(out[0, i], ref[0, i], 448.0 * 2.0 ** exps[i])
+
+
+@pytest.mark.parametrize("above", [20.6, 21.5, 23.4, 28.0, 40.0])
+@pytest.mark.parametrize("B,Sq,H,Hk,T,n", [(64, 1, 24, 24, 64, 4096), (64, 1, 8, 8, 16, 4095), (1, 20, 2, 2, 32, 250), (2, 1, 2, 1, 64, 9000)])
+def test_a_flat_tail_behind_one_key(dsb, cuda_dev, above, B, Sq, H, Hk, T, n):
+    """One key's score is `above` powers of two over all the others', which are equal, and its value is zero: what comes out is the
+    tail's values times 2^-above of their number, each probability with its 11 bits.
+
+    But for the keys that share a tile of 32 with that one key: their probabilities are rounded on the scale of its own, to a multiple
+    of 2^-24 where it is 2^12, so each is off by 2^-37 of it at most, and never by more than itself.  31 of n tail keys, of 2^-above
+    each: min(1, 2^(above - 37)) * 31 / (n - 1) of the result (values between 200 and 300 times their mean's 250: 1.2 of that)."""
+    from diffsynth_engine_b200 import kvcache
+    W = -(-n // T)
+    g = torch.Generator().manual_seed(n)
+    v = (torch.rand(W, Hk, T, 128, generator=g) * 100 + 200).to(torch.float8_e4m3fn)
+    k = torch.zeros(W, Hk, T, 128)
+    k[0, :, 3], v[0, :, 3] = 2.0, 0
+    k = k.to(torch.float8_e4m3fn)
+    q = torch.full((1, Sq, H, 128), 0.5).bfloat16()
+    scale = above * 0.6931471805599453 / 128                # the score is 128, and 2^above its power
+    ex = [torch.zeros(W, Hk, dtype=torch.int8), torch.full((W, Hk), -8, dtype=torch.int8)]
+    table = torch.arange(W, dtype=torch.int32)[None]
+    cache = kvcache.PagedKVCache(k.to(cuda_dev), v.to(cuda_dev), *(e.to(cuda_dev) for e in ex))
+    rows = OK.held(v.double(), ex[1], table[0], n)          # [n, Hk, 128]
+    w = torch.full((n,), 2.0 ** -above, dtype=torch.float64)
+    w[3] = 1
+    ref = torch.einsum("n,nhd->hd", w / w.sum(), rows).repeat_interleave(H // Hk, 0)[None, None].expand(B, Sq, H, 128)
+    out = kvcache.attend(q.expand(B, -1, -1, -1).to(cuda_dev), cache, table.expand(B, -1).contiguous().to(cuda_dev),
+                         torch.full((B,), n, dtype=torch.int32, device=cuda_dev), sm_scale=scale).double().cpu()
+    assert float(((out - ref).abs() / ref).max()) <= 2.0 ** -8 + 2.0 ** -11 + 1.2 * min(1, 2.0 ** (above - 37)) * 31 / (n - 1)  # (all values are positive)

@@ -64,4 +64,7 @@ DSB_HD int kv_exponent(uint32_t abs_bits) {
   return e < -64 ? -64 : (e > 64 ? 64 : e);
 }
 
+// A block's exponent as the kernels use it: what a caller has put there outside -64..64 counts as the nearer end.
+DSB_HD int kv_held_exponent(int e) { return e < -64 ? -64 : (e > 64 ? 64 : e); }
+
 }  // namespace dsb

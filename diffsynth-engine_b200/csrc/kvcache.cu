@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constan
     const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
     uint8_t* dst = (which ? p.pool.v : p.pool.k) + block * T * kD;
     int8_t* exps = (which ? p.pool.v_exp : p.pool.k_exp) + block;
-    const int was = *exps;
+    const int was = kv_held_exponent(*exps);
     uint4 raw[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) raw[c] = ahead[c];
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvRead p) {
   } else {
     const int64_t block = static_cast<int64_t>(page) * p.pool.heads + h;
     q = reinterpret_cast<const uint4*>((which ? p.pool.v : p.pool.k) + (block * T + tok % T) * kD)[c];
-    s = pow2i((which ? p.pool.v_exp : p.pool.k_exp)[block]);
+    s = pow2i(kv_held_exponent((which ? p.pool.v_exp : p.pool.k_exp)[block]));
   }
   const uint32_t u[4] = {q.x, q.y, q.z, q.w};
   uint32_t o[8];
@@ -540,7 +540,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
         for (int h = 0; h < 2; ++h) {
           x.k_exp[h] = x.v_exp[h] = 0;
           if (h == 1 && !T16) x.k_exp[1] = x.k_exp[0], x.v_exp[1] = x.v_exp[0];
-          else if (block[h] >= 0) x.k_exp[h] = p.pool.k_exp[block[h]], x.v_exp[h] = p.pool.v_exp[block[h]];
+          else if (block[h] >= 0 && key + 16 * h < c.ext)   // (a page that no key reaches may never have been written)
+            x.k_exp[h] = kv_held_exponent(p.pool.k_exp[block[h]]), x.v_exp[h] = kv_held_exponent(p.pool.v_exp[block[h]]);
         }
         x.unused[0] = block[0], x.unused[1] = block[1];
         infos[st][i % kInfoRing] = x;

@@ -19,7 +19,7 @@ PAGE_TOKENS = (16, 32, 64, 128)
 
 class PagedKVCache:
     """``k``, ``v``: float8_e4m3fn ``[pages, heads, T, 128]``; ``k_exp``, ``v_exp``: int8 ``[pages, heads]``, the power of two
-    that a block's values are multiplied by.  A page needs no preparation: the append that writes its first token sets its
+    that a block's values are multiplied by, -64 to 64 (others count as the nearer of the two).  A page needs no preparation: the append that writes its first token sets its
     exponent."""
 
     def __init__(self, k, v, k_exp, v_exp):

@@ -441,8 +441,10 @@ int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld_x, int x_b
 
 /*
  * Paged 8-bit cache of keys and values: k and v are e4m3 [n_pages, heads, page_tokens, 128] (contiguous, 128-byte aligned), k_exp
- * and v_exp one int8 per page and head: the values of that block are e4m3 * 2^exp.  page_tokens is 16, 32, 64 or 128, and
- * n_pages * heads * page_tokens is below 2^31.  `table` [B, ld_table] int32 names the `width` pages of each sequence in order.
+ * and v_exp one int8 per page and head: the values of that block are e4m3 * 2^exp, exp in -64..64 (anything else counts as the
+ * nearer end).  Neither the bytes nor the exponents of a page need be set before its first token is appended.  page_tokens is 16, 32,
+ * 64 or 128, and n_pages * heads * page_tokens is below 2^31.  `table` [B, ld_table] int32 names the `width` pages of each sequence in
+ * order.
  *
  * A table entry that is no page, a length or position outside the table or the rotation table: nothing is read or written
  * there (its keys count as masked, its rows are not appended, it reads as zeros) and *status becomes DSB_ERR_ARG.

@@ -1,5 +1,5 @@
 """Attention over the paged cache where its numbers lie far apart: value blocks of one sequence with very different exponents, one
-key far above a flat tail.
+key far above a flat tail, and exponents that no append has written.
 
 Tolerance: the output is rounded to bf16 (2^-8 of a value at most, 2^-8 / sqrt 3 rms), and each probability to 11 bits (2^-11), as in
 test_kvcache_gpu: 2^-8 + 2^-11 of each row's own norm, and per value 2^-8 of it plus 2^-10 of the largest value that the row
@@ -113,3 +113,44 @@ def test_a_flat_tail_behind_one_key(dsb, cuda_dev, above, B, Sq, H, Hk, T, n):
     out = kvcache.attend(q.expand(B, -1, -1, -1).to(cuda_dev), cache, table.expand(B, -1).contiguous().to(cuda_dev),
                          torch.full((B,), n, dtype=torch.int32, device=cuda_dev), sm_scale=scale).double().cpu()
     assert float(((out - ref).abs() / ref).max()) <= 2.0 ** -8 + 2.0 ** -11 + 1.2 * min(1, 2.0 ** (above - 37)) * 31 / (n - 1)  # (all values are positive)
+
+
+@pytest.mark.parametrize("garbage", [-128, -127, -65, 65, 127])
+@pytest.mark.parametrize("T", [16, 32])
+def test_exponents_of_unwritten_pages(dsb, cuda_dev, garbage, T):
+    """Pages need no preparation: their bytes and exponents may be anything until an append writes their first token."""
+    from diffsynth_engine_b200 import kvcache
+    lens = list(range(1, 2 * T + 2)) + [300, 333]
+    B, W = len(lens), -(-max(lens) // T) + 1
+    table = torch.arange(B * W, dtype=torch.int32).view(B, W)
+    g = torch.Generator().manual_seed(T)
+    k, v, q = (torch.randn(B, r, h, 128, generator=g).bfloat16() for r, h in ((max(lens), 1), (max(lens), 1), (2, 2)))
+    pools = [torch.full((B * W, 1, T, 128), 0x7f, dtype=torch.uint8, device=cuda_dev).view(torch.float8_e4m3fn) for _ in range(2)]
+    exps = [torch.full((B * W, 1), garbage, dtype=torch.int8, device=cuda_dev) for _ in range(2)]
+    cache = kvcache.PagedKVCache(*pools, *exps)
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    kvcache.append(cache, k.to(cuda_dev), v.to(cuda_dev), table.to(cuda_dev), 0, lt)
+    kv, ex = _held(cache)
+    ref = OK.attend(q, kv, ex, table, lens)
+    out = kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), lt)
+    _rows_near(out, ref, float(v.abs().max()) * 1.07)
+
+
+def test_exponents_outside_their_range(dsb, cuda_dev):
+    """A caller's exponents outside -64..64 count as the nearer end: for reads, attention and appends to the page."""
+    from diffsynth_engine_b200 import kvcache
+    g = torch.Generator().manual_seed(9)
+    kv = [(torch.randn(4, 2, 16, 128, generator=g) * 90).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in range(2)]
+    ex = [torch.tensor([[-128, 3], [127, -65], [0, 65], [-64, 100]], dtype=torch.int8), torch.tensor([[5, -128], [-100, 64], [127, 2], [65, -65]], dtype=torch.int8)]
+    q = torch.randn(1, 3, 2, 128, generator=g).bfloat16().to(cuda_dev)
+    rows = [(torch.randn(1, 5, 2, 128, generator=g) * s).bfloat16().to(cuda_dev) for s in (1e-3, 1e6)]
+    table = torch.arange(4, dtype=torch.int32, device=cuda_dev)[None]
+    got = []
+    for e in (ex, [t.clamp(-64, 64) for t in ex]):
+        cache = kvcache.PagedKVCache(*(t.to(cuda_dev) for t in kv), *(t.to(cuda_dev) for t in e))
+        out = [*kvcache.read(cache, table, 64), kvcache.attend(q, cache, table, 64)]
+        kvcache.append(cache, *rows, table, 57)
+        got.append(out + [cache.k[3].view(torch.uint8), cache.v[3].view(torch.uint8), cache.k_exp[3], cache.v_exp[3]])
+    assert all(torch.equal(a.nan_to_num(nan=7.0) if a.is_floating_point() else a, b.nan_to_num(nan=7.0) if b.is_floating_point() else b)
+               for a, b in zip(*got))
+    assert bool(got[0][0].isfinite().all()) and bool(got[0][1].isfinite().all())

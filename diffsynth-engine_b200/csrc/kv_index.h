@@ -67,4 +67,10 @@ DSB_HD int kv_exponent(uint32_t abs_bits) {
 // A block's exponent as the kernels use it: what a caller has put there outside -64..64 counts as the nearer end.
 DSB_HD int kv_held_exponent(int e) { return e < -64 ? -64 : (e > 64 ? 64 : e); }
 
+// Whether a stream's record of an item that goes on in the `more` streams behind it names an item and streams that there are; the combine
+// pass makes addresses of it.
+DSB_HD bool kv_cut_ok(int pair, int h, int more, int slot, int stream, int pairs, int heads, int n_streams) {
+  return pair >= 0 && pair < pairs && h >= 0 && h < heads && more > 0 && more < n_streams - stream && (slot == 0 || slot == 1);
+}
+
 }  // namespace dsb

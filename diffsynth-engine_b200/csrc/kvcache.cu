@@ -622,6 +622,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
     }
   }
   __syncthreads();
+  // (before the first wait: where one runs out, the combine pass finds nothing to do for this stream)
+  if (parts && sub == 0 && lane == 0) cuts[stream0 + st] = {-1, 0, 0, 0};
   const int n_mine = counts[st];
   const uint8_t* ring = rings + st * (kStages * kStageBytes);
 
@@ -950,7 +952,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) kv_attn_kernel(const __grid_c
       fresh = true;
     }
   }
-  if (parts && n_mine == 0 && sub == 0 && lane == 0) cuts[stream0 + st] = {-1, 0, 0, 0};
 }
 
 // Items that several streams shared are brought together from their parts (a stream's each), in order.  Where an item has a few
@@ -965,7 +966,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) kv_combine_kern
   int w0 = blockIdx.x;
   if constexpr (WARPS == 1) {
     cut = cuts[w0];
-    if (cut.pair < 0) return;
+    if (!kv_cut_ok(cut.pair, cut.h, cut.more, cut.slot, w0, work.pairs, work.heads, n_streams)) return;
   } else {
     cut.pair = work.by_heads(blockIdx.x);
     cut.h = blockIdx.x - cut.pair * work.heads;

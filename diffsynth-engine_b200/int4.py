@@ -79,12 +79,19 @@ def _check_weight(w):
         _require_cuda(w.payload)
 
 
+def _rows_apart(t):
+    """``t`` as rows that the kernels can step through: a copy where they overlap (a broadcast tensor)."""
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+
+
 def from_codes(codes, scales, mins=None, group=32) -> Int4Weight:
     """Lays out a weight that is quantised already: ``codes`` uint8 ``[N, K/2]`` (even column in the low nibble), ``scales`` and
     ``mins`` fp16 ``[N, ceil(K / group)]``."""
     _require_cuda(codes, scales, mins)
     if group not in GROUPS:
         raise _lib.DsbError(f"int4 groups are {GROUPS} columns, got {group}")
+    _rows(codes)
+    codes = _rows_apart(codes)
     N, half, ld = _rows(codes)
     K = 2 * half
     if codes.dtype != torch.uint8 or N == 0 or K == 0:
@@ -94,10 +101,10 @@ def from_codes(codes, scales, mins=None, group=32) -> Int4Weight:
             continue
         if t.dtype != torch.float16 or t.dim() != 2 or tuple(t.shape) != (N, -(-K // group)):
             raise _lib.DsbError(f"int4.from_codes {name} must be float16 [{N}, {-(-K // group)}], got {t.dtype} {tuple(t.shape)}")
-    if scales.stride(1) != 1 or (mins is not None and mins.stride() != scales.stride()):
+    if scales.stride(1) != 1 or _rows_apart(scales) is not scales or (mins is not None and mins.stride() != scales.stride()):
         scales, mins = scales.contiguous(), None if mins is None else mins.contiguous()
     w = _empty(N, K, group, mins is not None, codes.device)
-    rc = _lib.lib().dsb_int4_pack(_ptr(codes), ld, _ptr(scales), _ptr(mins), max(scales.stride(0), scales.shape[1]), N, K, group,
+    rc = _lib.lib().dsb_int4_pack(_ptr(codes), max(ld, half), _ptr(scales), _ptr(mins), max(scales.stride(0), scales.shape[1]), N, K, group,
                                   _ptr(w.payload), _ptr(w.scales), _ptr(w.mins), _stream())
     check(rc, "dsb_int4_pack")
     return w
@@ -109,6 +116,8 @@ def quantize_codes(W, group=32, asymmetric=False):
     _require_cuda(W)
     if group not in GROUPS:
         raise _lib.DsbError(f"int4 groups are {GROUPS} columns, got {group}")
+    _rows(W)
+    W = _rows_apart(W)
     N, K, ld = _rows(W)
     if W.dtype not in (torch.float32, torch.bfloat16) or N == 0 or K == 0 or K % 2:
         raise _lib.DsbError("int4.quantize takes fp32 or bf16 weights [N, K] with an even K")
@@ -135,6 +144,7 @@ def gguf_codes(raw, qtype: str):
     code, tsz, bsz = ops.GGUF_TYPES[qtype]
     if raw.dtype != torch.uint8 or raw.dim() != 2 or raw.stride(1) != 1 or raw.shape[0] == 0 or raw.shape[1] == 0 or raw.shape[1] % tsz:
         raise _lib.DsbError(f"int4.from_gguf({qtype}) takes uint8 rows of {tsz}-byte blocks")
+    raw = _rows_apart(raw)
     N, K = raw.shape[0], raw.shape[1] // tsz * bsz
     codes = torch.empty((N, K // 2), dtype=torch.uint8, device=raw.device)
     scales = torch.empty((N, K // 32), dtype=torch.float16, device=raw.device)

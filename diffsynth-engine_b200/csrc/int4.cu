@@ -292,10 +292,11 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 // time, which are then multiplied by the group's scale and added up in fp32.  Without minima A holds c - 8; with them it holds
 // c, and each group adds m * (sum of its activations).
 //
-// The activations keep their precision: a row is scaled by a power of two that brings its largest magnitude to [2^13, 2^14).  A
-// bf16 value is then exact in fp16 unless it is less than 2^-27 of that; an fp32 value (and a bf16 one behind an activation)
-// becomes two columns (SPLIT), high = fp16(x) and low = fp16(x - high), which leaves out 2^-23 of it at most, what one fp32
-// rounding of a product would.
+// The activations keep their precision: a row (of a share of the columns) is scaled by a power of two that brings its largest
+// magnitude to [2^13, 2^14).  A bf16 value is then exact in fp16 if it is at least 2^-30 of that; a smaller one is off by 2^-25, that is
+// 2^-38 of the largest, at most.  An fp32 value (and a bf16 one behind an activation) becomes two columns (SPLIT), high = fp16(x) and
+// low = fp16(2^12 (x - high)), whose sums are kept apart until the end: x - high is 2^2 at most, so low stays below 2^14.  That leaves
+// out 2^-23 of the value, what one fp32 rounding of a product would, or 2^-25 / 2^12, which is 2^-50 of the largest, whichever is more.
 //
 // Split: a cluster of `n_share` CTAs owns a range of row blocks, each CTA a share of the columns, whose activations are all that
 // it stages; a warp takes every eighth row block of the range and streams its tiles without a pause from one to the next.
@@ -310,6 +311,7 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 // barrier (small 2.9, large 275).
 constexpr int kGemvSmemMax = 227 * 1024 - 1024;
 constexpr int kGemvCtas = 2;  // per SM
+constexpr float kLowUp = 4096.f;  // what a low column is multiplied by
 constexpr int kBatch = 4;  // tiles of a warp in one of the two register buffers that the loads in flight fill
 
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
       if constexpr (SPLIT) {
         // (an infinity is its high part alone)
         const float ra = fabsf(a) < INFINITY ? a - __low2float(h) : 0.f, rb = fabsf(b) < INFINITY ? b - __high2float(h) : 0.f;
-        const __half2 l = __floats2half2_rn(ra, rb);
+        const __half2 l = __floats2half2_rn(ra * kLowUp, rb * kLowUp);
         lo[j] = *reinterpret_cast<const uint32_t*>(&l);
       }
     }
@@ -570,7 +572,7 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
         for (int c = 0; c < (SPLIT ? 1 : 2); ++c) {
           const int m = SPLIT ? n * 4 + t : n * 8 + 2 * t + c, row = g + 8 * r;
           if (m < p.M) {
-            const float v = (SPLIT ? acc[n][2 * r] + acc[n][2 * r + 1] : acc[n][2 * r + c]) * up[m].x * up[m].y;
+            const float v = (SPLIT ? fmaf(acc[n][2 * r + 1], 1.f / kLowUp, acc[n][2 * r]) : acc[n][2 * r + c]) * up[m].x * up[m].y;
             if constexpr (CLUSTERED)
               red[(block * p.M + m) * 16 + row] = v;
             else if ((round0 + block) * 16 + row < d.N)

@@ -433,7 +433,8 @@ int dsb_int4_dequant(const dsb_int4_weight* w, void* out, int64_t ld_out, void* 
 /*
  * y = act_out(W . act_in(x) + bias) (+ y before, with `accumulate`) for M <= DSB_INT4_MAX_ROWS rows x[M, ld_x] (fp32 or bf16; any
  * alignment of its type) and a laid-out 4-bit W; products and sums in fp32; y fp32 or bf16.  act_in is NONE or SILU.  y must
- * not overlap x.
+ * not overlap x.  Of an act_in(x) the products leave out 2^-23 of it at most, or 2^-50 of the row's largest magnitude if that is more
+ * (bf16 rows without act_in: nothing, or 2^-38 of the largest).
  */
 #define DSB_INT4_MAX_ROWS 32
 int dsb_gemv_int4(const dsb_int4_weight* w, const void* x, int64_t ld_x, int x_bf16, const float* bias, void* y, int64_t ld_y,

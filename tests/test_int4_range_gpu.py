@@ -1,4 +1,4 @@
-"""4-bit weights at the borders of their calls: rows shared in memory.
+"""4-bit weights at the borders of their calls: rows shared in memory, activations that lie far apart.
 
 Tolerances as in test_int4_gpu: 2e-6 of the norm for fp32 results; half a bf16 step, 2^-8, where operands or results are rounded to
 bf16."""
@@ -36,3 +36,22 @@ def test_rows_shared_by_broadcasting(dsb, cuda_dev, group, mins):
     W = torch.randn(1, K, generator=torch.Generator().manual_seed(3)).to(cuda_dev).expand(N, K)
     for a, b in zip(int4.quantize_codes(W, group, mins), int4.quantize_codes(W.contiguous(), group, mins)):
         assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+@pytest.mark.parametrize("outlier", [2.0 ** 20, 2.0 ** 27])
+@pytest.mark.parametrize("N,K,M", [(64, 256, 1), (200, 1026, 3), (3000, 320, 9)])
+@pytest.mark.parametrize("silu", [False, True])
+def test_small_activations_beside_an_outlier(dsb, cuda_dev, outlier, N, K, M, silu):
+    """Outputs whose weight is zero at a row's outlier are made of its small activations alone, and as good as they would be without it."""
+    from diffsynth_engine_b200 import int4, ops
+    c, s, _ = _weight(N, K, 32, False, K)
+    at = K // 2 & ~1
+    c[:, at // 2] = c[:, at // 2] & 0xf0 | 8
+    w = int4.from_codes(*_on(cuda_dev, c, s), group=32)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M))
+    x[:, at] = outlier
+    y = int4.gemv(w, x.to(cuda_dev), act_in=ops.ACT_SILU if silu else ops.ACT_NONE).cpu()
+    x[:, at] = 0
+    ref = O4.linear(x, O4.values(c, s, None, 32), act_in=torch.nn.functional.silu if silu else None)
+    for got, want in zip(y, ref):
+        assert O.rel_l2(got, want) < 2e-6

@@ -320,6 +320,32 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
+// The product of columns k0 .. k1 - 1 of an activation row m that has infinities there with row `row` of a row block of a weight with
+// minima: an infinity of the sign that s c + m has, or NaN, and no other column but a NaN matters.  (c and m on their own have other
+// signs, so the tensor cores' sums are no use.)  All lanes of a warp, each with a row.  Not inlined: a rare case that should not cost
+// the others registers.
+__device__ __noinline__ float infinite_part(Int4Dims d, GemvInt4 p, int64_t row_block, int row, int m, int k0, int k1) {
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.payload);
+  float sum = 0.f;
+  for (int base = k0; base < k1; base += 32) {
+    const int mine = base + (threadIdx.x & 31);
+    float x = 0.f;
+    if (mine < k1) {
+      const int64_t at = m * p.ld_x + mine;
+      x = p.x_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.x)[at]) : reinterpret_cast<const float*>(p.x)[at];
+      if (p.act_in == DSB_ACT_SILU) x = silu(x);
+    }
+    for (uint32_t hits = __ballot_sync(0xffffffffu, !(fabsf(x) < INFINITY)); hits; hits &= hits - 1) {
+      const int src = __ffs(hits) - 1, k = base + src;
+      const int j = 2 * ((k >> 5) & 1) + ((k >> 2) & 1), lane = 4 * (row & 7) + ((k >> 3) & 3), nibble = (row >> 3) + (k & 2) + 4 * (k & 1);
+      const uint32_t code = words[((row_block * d.k_tiles + (k >> 6)) * 32 + lane) * 4 + j] >> (4 * nibble) & 15u;
+      const int64_t si = scale_index(d, row_block, row, k);
+      sum += (__half2float(p.scales[si]) * static_cast<float>(code) + __half2float(p.mins[si])) * __shfl_sync(0xffffffffu, x, src);
+    }
+  }
+  return sum;
+}
+
 template <int NT, bool SPLIT, int GROUP, bool MINS, bool CLUSTERED>
 __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, GemvInt4 p, int n_share, int share_tiles, int round_blocks) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -333,12 +359,13 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
   uint8_t* xs = smem;                                               // [cols] rows of fp16
   float* xsum = reinterpret_cast<float*>(xs + cols * x_pitch);      // [share_groups][kRows]
   float* red = xsum + kRows * share_groups;                         // CLUSTERED: [round_blocks][M][16 rows]
-  __shared__ uint32_t amax_bits[kRows];
+  __shared__ uint32_t amax_bits[kRows], inf_rows;   // (a bit for each activation row that has infinities; with minima)
   __shared__ float2 up[kRows];  // the power of two that a row's sums are multiplied by, as two factors
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = CLUSTERED ? cluster_ctarank() : 0;
   const int n_ranges = CLUSTERED ? gridDim.x / n_share : gridDim.x, range = CLUSTERED ? blockIdx.x / n_share : blockIdx.x;
   if (tid < kRows) amax_bits[tid] = 0;
+  if (MINS && tid == 0) inf_rows = 0;
   grid_wait();
   const int tile0 = rank * share_tiles;
   const int n_tiles = max(0, min(share_tiles, d.k_tiles - tile0));   // of this share in every row block
@@ -433,12 +460,23 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
   auto largest = [&](int m, const float (&v)[8]) {  // of a warp's finite magnitudes, into the row's
     float a = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (fabsf(v[j]) < INFINITY) a = fmaxf(a, fabsf(v[j]));
+    for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(v[j]));   // (not of a NaN)
+    if (a == INFINITY) {
+      a = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(v[j]) < INFINITY) a = fmaxf(a, fabsf(v[j]));
+      if (MINS) atomicOr(&inf_rows, 1u << m);
+    }
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(a));
     if (lane == 0) atomicMax(&amax_bits[m], bits);
   };
-  auto convert = [&](int m, int e8, bool in, const float (&v)[8]) {
+  auto convert = [&](int m, int e8, bool in, float (&v)[8]) {
+    if (MINS && (inf_rows >> m & 1)) {   // (see infinite_part)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(v[j]) == INFINITY) v[j] = 0.f;
+    }
     // the power of two, as two factors: its exponent may pass 127
     const uint32_t top = amax_bits[m];
     const int e = top ? ilogbf(__uint_as_float(top)) - 13 : 0, half = e / 2;
@@ -564,6 +602,7 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
   };
   // the sums of a finished row block (its number in the round)
   auto finish = [&](int block) {
+    const uint32_t later = MINS && !CLUSTERED ? inf_rows : 0;   // (rows with infinities have their results from infinite_part)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -571,7 +610,7 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
 #pragma unroll
         for (int c = 0; c < (SPLIT ? 1 : 2); ++c) {
           const int m = SPLIT ? n * 4 + t : n * 8 + 2 * t + c, row = g + 8 * r;
-          if (m < p.M) {
+          if (m < p.M && !(later >> m & 1)) {
             const float v = (SPLIT ? fmaf(acc[n][2 * r + 1], 1.f / kLowUp, acc[n][2 * r]) : acc[n][2 * r + c]) * up[m].x * up[m].y;
             if constexpr (CLUSTERED)
               red[(block * p.M + m) * 16 + row] = v;
@@ -613,6 +652,20 @@ __global__ void __launch_bounds__(256, kGemvCtas) gemv_int4_kernel(Int4Dims d, G
       load(0);
       multiply(1);
       load(1);
+    }
+    if (MINS && inf_rows) {
+      __syncwarp();
+      for (int at = warp; at < in_round; at += 8)
+        for (uint32_t rows = inf_rows; rows; rows &= rows - 1) {
+          const int m = __ffs(rows) - 1, row = lane & 15;
+          const float part = infinite_part(d, p, round0 + at, row, m, tile0 * 64, min(d.K, (tile0 + n_tiles) * 64));
+          if (lane < 16) {
+            if constexpr (CLUSTERED)
+              red[(at * p.M + m) * 16 + row] = part;
+            else if ((round0 + at) * 16 + row < d.N)
+              emit(m, (round0 + at) * 16 + row, part);
+          }
+        }
     }
     const int next = round0 + in_round, next_in = min(round_blocks, block1 - next);
     if constexpr (CLUSTERED) {

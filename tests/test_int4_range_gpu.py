@@ -1,4 +1,4 @@
-"""4-bit weights at the borders of their calls: rows shared in memory, activations that lie far apart.
+"""4-bit weights at the borders of their calls: rows shared in memory, activations that lie far apart or are not finite.
 
 Tolerances as in test_int4_gpu: 2e-6 of the norm for fp32 results; half a bf16 step, 2^-8, where operands or results are rounded to
 bf16."""
@@ -55,3 +55,37 @@ def test_small_activations_beside_an_outlier(dsb, cuda_dev, outlier, N, K, M, si
     ref = O4.linear(x, O4.values(c, s, None, 32), act_in=torch.nn.functional.silu if silu else None)
     for got, want in zip(y, ref):
         assert O.rel_l2(got, want) < 2e-6
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,K", [(70, 192), (200, 1026), (5000, 320)])
+def test_infinite_activations(dsb, cuda_dev, group, mins, dtype, N, K):
+    """A row with infinities gives what the products of its weights give: infinities of the weights' signs, NaN where the weight is
+    zero or the signs disagree; the other rows are as ever."""
+    from diffsynth_engine_b200 import int4, ops
+    c, s, m = _weight(N, K, group, mins, N + K)
+    if mins:
+        s[3], m[3] = 0.0078125, -0.015625           # code 2 is a zero
+    w = int4.from_codes(*_on(cuda_dev, c, s, m), group=group)
+    W = O4.values(c, s, m, group)
+    x = torch.randn(12, K, generator=torch.Generator().manual_seed(1))
+    inf = float("inf")
+    x[0, 5], x[2, K - 1], x[3, 40], x[3, 41] = inf, -inf, inf, inf
+    x[4, 7], x[4, K - 2], x[5, 0], x[5, 33], x[5, K // 2] = inf, -inf, -inf, -inf, -inf
+    x[7, 9], x[7, 10] = inf, float("nan")
+    x[9, ::3] = inf
+    x = x.to(dtype)
+    for act, f in ((ops.ACT_NONE, None), (ops.ACT_SILU, lambda t: torch.where(t == -inf, 0.0, t * torch.sigmoid(t)))):
+        y = int4.gemv(w, x.to(cuda_dev), act_in=act, out=torch.empty(12, N, device=cuda_dev)).cpu()
+        if f is not None:       # (the activation of -infinity is NaN or 0, as 0 * -inf is taken)
+            keep = ~(x == -inf).any(1)
+        else:
+            keep = torch.ones(12, dtype=torch.bool)
+        ref = O4.linear(x, W, act_in=f)
+        y, ref = y[keep], ref[keep]
+        assert torch.equal(y.isnan(), ref.isnan())
+        assert torch.equal(y.isposinf(), ref.isposinf()) and torch.equal(y.isneginf(), ref.isneginf())
+        rows = ref.isfinite().all(1)
+        assert rows.sum() >= 5 and O.rel_l2(y[rows], ref[rows]) < 2e-6

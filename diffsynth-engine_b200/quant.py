@@ -139,6 +139,22 @@ def enable_b200_linear(module: nn.Module, fmt: str = "fp8_tensor"):
     setattr(module, "b200_linear_enabled", True)
 
 
+def _int4_gemm(x, w4: int4.Int4Weight, bias):
+    """``x @ W.T + bias`` of many rows with a 4-bit weight, which is expanded to bf16 for the GEMM.  The GEMM takes rows that are
+    multiples of 16 bytes apart and a multiple of 8 outputs: other widths are padded, and the outputs cut."""
+    N, K = w4.N, w4.K
+    n8, k8 = -(-N // 8) * 8, -(-K // 8) * 8
+    xb = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
+    if xb.stride(-1) != 1 or (xb.stride(0) % 8) or (xb.data_ptr() % 16) or xb.stride(0) < K:
+        xb = torch.empty((x.shape[0], k8), dtype=torch.bfloat16, device=x.device)[:, :K].copy_(xb) if k8 != K else xb.contiguous()
+    if (n8, k8) == (N, K):
+        return ops.gemm(xb, int4.dequant(w4), bias=bias)
+    w = torch.empty((n8, k8), dtype=torch.bfloat16, device=x.device)[:, :K]     # (columns past K are not read, rows past N not used)
+    int4.dequant(w4, out=w[:N])
+    y = ops.gemm(xb, w, bias=bias if bias is None or n8 == N else F.pad(bias, (0, n8 - N)))
+    return y if n8 == N else y[:, :N].contiguous()
+
+
 def b200_linear(input: torch.Tensor, weight: torch.Tensor, bias=None, _origin=F.linear) -> torch.Tensor:
     """``F.linear`` for a ``QuantLinearWeight``: flatten leading dims, quantise rows, tensor-core GEMM with the
     scales and bias in its epilogue, output in the input dtype (the dataflow of utils/fp8_linear.py:27-60)."""
@@ -157,10 +173,7 @@ def b200_linear(input: torch.Tensor, weight: torch.Tensor, bias=None, _origin=F.
             xf = x if x.dtype in (torch.bfloat16, torch.float32) else x.float()
             y = int4.gemv(w4, xf if xf.stride(-1) == 1 and xf.stride(0) >= K else xf.contiguous(), b32)
         else:
-            xb = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
-            if xb.stride(-1) != 1 or (xb.stride(0) % 8) or (xb.data_ptr() % 16):
-                xb = xb.contiguous()
-            y = ops.gemm(xb, int4.dequant(w4), bias=b32)
+            y = _int4_gemm(x, w4, b32)
     elif ext is None and M <= 4:
         # conditioning vectors: bandwidth-bound GEMV on fp32 activations, weights dequantised on the fly
         xf = x if x.dtype in (torch.bfloat16, torch.float32) else x.float()

@@ -1,4 +1,5 @@
-"""4-bit weights at the borders of their calls: rows shared in memory, activations that lie far apart or are not finite.
+"""4-bit weights at the borders of their calls: rows shared in memory, activations that lie far apart or are not finite, Linears
+of odd widths.
 
 Tolerances as in test_int4_gpu: 2e-6 of the norm for fp32 results; half a bf16 step, 2^-8, where operands or results are rounded to
 bf16."""
@@ -89,3 +90,26 @@ def test_infinite_activations(dsb, cuda_dev, group, mins, dtype, N, K):
         assert torch.equal(y.isposinf(), ref.isposinf()) and torch.equal(y.isneginf(), ref.isneginf())
         rows = ref.isfinite().all(1)
         assert rows.sum() >= 5 and O.rel_l2(y[rows], ref[rows]) < 2e-6
+
+
+@pytest.mark.parametrize("N,K", [(72, 256), (70, 256), (72, 258), (70, 258), (1, 2), (9, 34)])
+@pytest.mark.parametrize("M", [32, 33, 140])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linears_of_odd_widths(dsb, cuda_dev, N, K, M, bias):
+    """A Linear that 32 rows can go through takes any number."""
+    from diffsynth_engine_b200 import quant
+    layer = torch.nn.Linear(K, N, bias=bias).to(cuda_dev)
+    W = O4.values(*O4.quantize(layer.weight.data.cpu(), 32, True), 32)
+    quant.enable_b200_linear(layer, "int4_group")
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(2 * M, K + 1, device=cuda_dev).to(dtype)
+        for rows in (x[:M, :K], x[::2, 1:], x[:M, :K].reshape(1, M, K), x[:1, :K].expand(M, K)):
+            with quant.b200_inference():
+                got = layer(rows)
+            assert got.shape == (*rows.shape[:-1], N) and got.dtype == dtype and got.is_contiguous()
+            xr, W_ = rows.reshape(-1, K).cpu(), W
+            if M > 32:
+                xr, W_ = xr.bfloat16(), W.bfloat16()
+            ref = O4.linear(xr, W_, layer.bias.detach().cpu() if bias else None)
+            tol = 2e-6 if M <= 32 and dtype == torch.float32 else 2.0 ** -8 * 1.05
+            assert O.rel_l2(got.detach().reshape(-1, N).cpu(), ref) < tol

@@ -154,3 +154,30 @@ def test_exponents_outside_their_range(dsb, cuda_dev):
     assert all(torch.equal(a.nan_to_num(nan=7.0) if a.is_floating_point() else a, b.nan_to_num(nan=7.0) if b.is_floating_point() else b)
                for a, b in zip(*got))
     assert bool(got[0][0].isfinite().all()) and bool(got[0][1].isfinite().all())
+
+
+def test_pages_only(dsb, cuda_dev, monkeypatch):
+    """Whatever the estimate says: the pages' own precision, and keys of entries that are no pages masked."""
+    from diffsynth_engine_b200 import kvcache
+    g = torch.Generator().manual_seed(4)
+    B, Sq, H, T, W = 2, 600, 2, 64, 5
+    kv = [(torch.randn(B * W, H, T, 128, generator=g) * 90).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in range(2)]
+    ex = [torch.full((B * W, H), -7, dtype=torch.int8) for _ in range(2)]
+    cache = kvcache.PagedKVCache(*(t.to(cuda_dev) for t in kv), *(t.to(cuda_dev) for t in ex))
+    q = torch.randn(B, Sq, H, 128, generator=g).bfloat16()
+    table = torch.randperm(B * W, generator=g).view(B, W).int()
+    monkeypatch.setattr(kvcache, "dense_pays", lambda *sizes: True)
+    n = W * T - 3
+    out = kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), n, pages_only=True)
+    lens = torch.full((B,), n, dtype=torch.int32, device=cuda_dev)
+    assert torch.equal(out, kvcache.attend(q.to(cuda_dev), cache, table.to(cuda_dev), lens))
+    top = float(max((t.double().abs().max() for t in kv))) * 2.0 ** -7
+    _rows_near(out, OK.attend(q, [t.double() for t in kv], ex, table, [n] * B), top)
+    bad = table.clone()
+    bad[1, 2] = B * W
+    out = kvcache.attend(q.to(cuda_dev), cache, bad.to(cuda_dev), n, pages_only=True)
+    with pytest.raises(dsb.DsbError, match="ERR_ARG"):
+        dsb.ops.check_status(0)
+    seen = torch.ones(B, n, dtype=torch.bool)
+    seen[1, 2 * T:3 * T] = False
+    _rows_near(out, OK.attend(q, [t.double() for t in kv], ex, table, [n] * B, ok=seen), top)

@@ -260,8 +260,8 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-// Eight codes of a word as four pairs of fp16 numbers c - 8 (or c), exact: a code in the mantissa of 1024 is 1024 + c in its low four
-// bits and 1024 + 16 c in the next four, so that one shift serves four pairs.
+// Eight codes of a word as four pairs of fp16 numbers c - 8 (or c), exact, in the way that is usual for 4-bit weights: a code in the
+// mantissa of 1024 is 1024 + c in its low four bits and 1024 + 16 c in the next four, so that one shift serves four pairs.
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {  // one instruction; the compiler makes two of it
   uint32_t d;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
@@ -302,10 +302,12 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
 // it stages; a warp takes every eighth row block of the range and streams its tiles without a pause from one to the next.
 // Shares meet in shared memory (CLUSTERED), in a fixed order.
 //
-// Bound by the bytes of the weight where there are many: 491520 x 5120 in groups of 32 takes 261 us (5.4 of 6.55 TB/s); 66
-// instructions for 512 bytes, 20 of them logic (one lop3 for two codes: written as and + or it is two, 292 us).  Small ones are
-// latency: 768 x 256 takes 3.4 us, 5120 x 5120 10.8 (2.5 at the copy rate): launch 2, activations 1.2, then a few batches of loads
-// and cold code, 1.6 for the two cluster barriers.  Tried and not kept: a cp.async ring instead of register buffers (342 us for the
+// Bound by the bytes of the weight where there are many: 491520 x 5120 in groups of 32 takes 265 us (5.4 of 6.55 TB/s) in bursts of
+// some 40 launches and 300 when they go on for half a second, at 880 W and unchanged clocks, whether the weight is the same or another;
+// 66 instructions for 512 bytes, 20 of them logic (one lop3 for two codes: written as and + or it is two, 292 us).  Small ones are
+// latency: 768 x 256 takes 3.7 us, 5120 x 5120 9.5 to 10.5 (2.5 at the copy rate), with minima 11.8: launch 2, activations 1.2, then a few
+// batches of loads and cold code, 1.6 for the two cluster barriers.  An e4m3 weight (one byte each, gemv_kernel) takes 12.7 at 5120 x
+// 5120, 16.6 at 13824 x 5104 (here 17.2, with minima 19.4) and 385 at 491520 x 5120.  Tried and not kept: a cp.async ring instead of register buffers (342 us for the
 // large one), a third CTA per SM (80 registers: spills), each register slot refilled as it is used (the waits share scoreboards:
 // 622 with minima), equal runs of tiles for the warps instead of row blocks (+5 %), sums pushed into the owner's memory to save a
 // barrier (small 2.9, large 275).
@@ -754,9 +756,10 @@ static int run_gemv_int4(const Int4Dims& d, const GemvInt4& p, int n_share, cuda
 template <int NT, bool SPLIT, int GROUP, bool MINS>
 static int launch_gemv_int4(const Int4Dims& d, const GemvInt4& p, cudaStream_t st) {
   // Shares of the columns, of four tiles at least.  Each costs a CTA less staging and evens out the work, and a pass over the
-  // sums through distributed shared memory.  Measured (us; 1, 2, 4, 8 shares): 5120 x 5120 20.2 13.4 10.8 10.9, 13827 x 5104 with
-  // five rows 25.7 20.6 17.7 17.9, with 16 rows 52 35 26 25, 30720 x 5120 25.4 23.9 23.5 25.5, 491520 x 5120 261 253 269 316 and
-  // with minima 269 279 301 342.  Weights with fewer row blocks than four shares need to reach every SM take eight.
+  // sums through distributed shared memory.  Measured (us; 1, 2, 4, 8 shares): 5120 x 5120 18.2 11.5 9.5 9.6, 13827 x 5104 with
+  // minima and five rows 29.9 21.9 18.6 18.3, with 16 rows 67.9 42.9 30.1 28.0, 30720 x 5120 26.5 24.7 23.9 25.9, 491520 x 5120 263 253
+  // 273 309, with minima 323 329 334 366, and 1056768 x 48 tiles with minima 416 420 440 512.  Weights with fewer row blocks than four
+  // shares need to reach every SM take eight, the largest one: two would be 4 % less without minima and 1 to 2 % more with them.
   int n_share = d.row_blocks * 4 < 8 * sm_count() ? 8 : 4;
   while (n_share > 1 && d.k_tiles < 4 * n_share) n_share /= 2;
   if (d.row_blocks >= 16 * 8 * sm_count()) n_share = 1;

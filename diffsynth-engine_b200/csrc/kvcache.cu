@@ -60,8 +60,8 @@ struct KvAppend {
 // way.  The (cos, sin) of the rows are fetched once, into shared memory, and every key is rotated twice: for the exponent, and
 // to be written.  CHUNKS: loads of a thread for a whole page.
 //
-// Bound by the bytes: 256 in and 128 out for a row of a head.  Measured (us): 2 x about 4700 tokens of 40 heads, rotated, 62 (47 at
-// the copy rate); with a CTA for each head, rotations read from L2 by each and kept in fp32 registers, 83; the same with 256
+// 256 bytes in and 128 out for a row of a head.  Measured (us): 2 x about 4700 tokens of 40 heads, rotated, 59 to 62 (47 at the copy
+// rate), with 73 % of the issue slots of a busy SM taken (rotation and rounding) and 2.1 waves of CTAs at five an SM, a quarter of them without rows; with a CTA for each head, rotations read from L2 by each and kept in fp32 registers, 83; the same with 256
 // threads a CTA 81 (pages of 64 tokens) to 131 (16); with each magnitude compared with infinity 69.  512 tokens 5 to 7, one token of
 // 16 sequences 3: latency.
 template <int THREADS, int CHUNKS, bool ROTATE>
@@ -303,16 +303,18 @@ struct KvAttn {
 // and moves only when a t is 2^kHigh above it (moving it with every new maximum cost a rescaling of O in about every second tile), and
 // a tile whose largest p of a row is below 2^-kLow - a flat tail behind one large score, or values far smaller than another
 // block's - is multiplied apart: p relative to its own largest t, and P V brought to the row's scale and added to O in fp32.  What
-// rounding leaves out of a p is at most 2^-12 of it, or 2^-25 / 2^-kLow = 2^-15 of the largest p of its row and tile (of its half
+// rounding leaves out of a p is at most 2^-11 of it, or 2^-25 / 2^-kLow = 2^-15 of the largest p of its row and tile (of its half
 // of the tile, where the halves are of two pages).
 //
 // What bounds it: one row tile per cache head (a token of each sequence) the cache's bytes, behind about 10 us of start (lengths,
 // page table, first tiles, and code that no cache holds yet) and 4 for the combine pass.  A warp's tile takes about 2500 cycles
 // (S 780, softmax 560, P V 800, each a chain of dependent steps), and eight warps an SM are just what the memory rate needs; more
 // warps would halve the registers.  With more rows the same chains bind: 64 rows share a ring, but each warp converts for itself.
-// Measured (us): 77 keys x 24 heads 8; 16 ragged sequences of up to 16384 keys, 8 cache heads 70 (48 at the copy rate); 2 x 131071
-// keys, 32 rows 85 (32); 3 x 260 queries over ragged 8100 keys 456 (54 at the tensor rate of tcgen05, which mma.sync does not
-// reach).  Tried and slower: fragments of V made before the softmax and S in two sums (spills; 75 instead of 71), ten warps with
+// Measured (us): 77 keys x 24 heads 8; 16 ragged sequences of up to 16384 keys, 8 cache heads 71 (48 at the copy rate); 2 x 131071
+// keys, 32 rows 83 (32); 3 x 260 queries over ragged 8100 keys 465 (54 at the tensor rate of tcgen05, which mma.sync does not
+// reach).  Without a look at what falls below fp16 the last three are 70, 77 and 433, and wrong where something does; of the difference
+// kLow = 10 instead of 13, with which a tile's small p could lose eight times as much, makes 0, 3 and 12.
+// Tried and slower, before that: fragments of V made before the softmax and S in two sums (spills; 75 instead of 71), ten warps with
 // shorter rings (same; short calls +1), and converting each tile once for all its warps through shared memory, by warps of its own
 // (137 and 518 instead of 87 and 468) or by the consumers in parts (128 and 661).
 constexpr int kTile = 32;       // keys

@@ -164,7 +164,7 @@ def workspace_bytes(device: int) -> int:
 
 def dense_pays(batch: int, queries: int, heads: int, cache_heads: int, tokens: int) -> bool:
     """Whether ``attend`` gathers the sequences as bf16 rows for the dense attention kernel, instead of reading the pages: an estimate
-    of both in microseconds.  Pages: 9, 9 more where sequences may be cut, and 210 Mflop a microsecond.  Dense: 8 for the gather (4
+    of both in microseconds, from times on one B200 (148 SMs).  Pages: 9, 9 more where sequences may be cut, and 210 Mflop a microsecond.  Dense: 8 for the gather (4
     on the device, but two calls' arguments) and its bytes, then for each query head of a group one launch of items of 256 rows, 74 at
     a time, each 2.4 and 0.62 a tile of 128 keys; one cache head's query heads are rows of one launch.  Measured on the device (pages,
     dense; heads / cache heads, queries x tokens): 24/24 256 x 77: 9, 13; 256 x 512: 24, 16; 4096 x 4096: 925, 190; 32/8 512 x 512:

@@ -310,10 +310,10 @@ struct KvAttn {
 // page table, first tiles, and code that no cache holds yet) and 4 for the combine pass.  A warp's tile takes about 2500 cycles
 // (S 780, softmax 560, P V 800, each a chain of dependent steps), and eight warps an SM are just what the memory rate needs; more
 // warps would halve the registers.  With more rows the same chains bind: 64 rows share a ring, but each warp converts for itself.
-// Measured (us): 77 keys x 24 heads 8; 16 ragged sequences of up to 16384 keys, 8 cache heads 71 (48 at the copy rate); 2 x 131071
-// keys, 32 rows 83 (32); 3 x 260 queries over ragged 8100 keys 465 (54 at the tensor rate of tcgen05, which mma.sync does not
-// reach).  Without a look at what falls below fp16 the last three are 70, 77 and 433, and wrong where something does; of the difference
-// kLow = 10 instead of 13, with which a tile's small p could lose eight times as much, makes 0, 3 and 12.
+// Measured (us): 77 keys x 24 heads 8; 16 ragged sequences of up to 16384 keys, 8 cache heads 70 (48 at the copy rate); 2 x 131071
+// keys, 32 rows 80 (32); 3 x 260 queries over ragged 8100 keys 454 (54 at the tensor rate of tcgen05, which mma.sync does not
+// reach).  Without a look at what falls below fp16 the last three are 70, 77 and 433, and wrong where something does; with kStart = 12 and
+// kHigh = 15, two powers of two less room, 71, 83 and 465 (more tiles are looked at closely, for no more than that).
 // Tried and slower, before that: fragments of V made before the softmax and S in two sums (spills; 75 instead of 71), ten warps with
 // shorter rings (same; short calls +1), and converting each tile once for all its warps through shared memory, by warps of its own
 // (137 and 518 instead of 87 and 468) or by the consumers in parts (128 and 661).
@@ -327,7 +327,7 @@ constexpr int kStageBytes = 2 * kTile * kD;
 constexpr int kAttnRing = kAttnWarps * kAttnStages * kStageBytes;
 constexpr int kAttnDynSmem = kAttnRing + 1024;
 constexpr int kMinShare = DSB_KV_UNCUT_TOKENS / kTile;  // tiles: fewer are not worth another warp
-constexpr float kStart = 12.f, kHigh = 15.f, kLow = 10.f;
+constexpr float kStart = 13.f, kHigh = 15.9f, kLow = 10.f;
 constexpr int kPartRow = 132;   // floats of a partial row: 128 columns, reference exponent, sum, two unused
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
